@@ -257,6 +257,74 @@ int ishz_moe_swiglu(uint32_t type, const void *x, int x_dtype, int T, int H, con
                     const void *shared_gate, void *y, int32_t *ids_out, float *weights_out,
                     void *workspace, size_t workspace_bytes, ishz_stream_t stream);
 
+/* ---------------------------------------------------------------- attention over an 8-bit cache
+ * What a decoder layer does between its qkv projection and its output projection.
+ *
+ * Activations are [rows][heads][dim] with any stride between rows and between heads (in values; rows
+ * and heads start on 16 bytes), so q, k and v may be parts of one projection's output. dim is 64, 128
+ * or 256; fp32, fp16 or bf16 (attention's q: fp16 or bf16). Other dims and dtypes are declined.
+ *
+ * The cache is a pool of blocks of ISHZ_KV_BLOCK tokens. Codes: of keys [blocks][heads][64][dim], of
+ * values [blocks][heads][dim][64], one byte each; scales [blocks][heads] fp32 of either. A value is its
+ * code times its block's and head's scale.
+ *
+ * A call's sequences: table [sequences][width] holds each sequence's block numbers in order, lengths
+ * [sequences] its tokens in the cache, the call's own among them, and starts [sequences + 1] the first of
+ * its rows, so sequence s has rows starts[s] .. starts[s+1] - 1 at positions lengths[s] - n .. lengths[s] - 1
+ * of its cache. All three are device memory, read by the kernels, so that a captured call follows them as
+ * they change. A sequence may have no rows, or no tokens. An entry of the table outside the pool holds no
+ * tokens: what would be written there is dropped, attention leaves it out and reading gives zeros (so blocks
+ * behind a window may be freed). Tokens past `width` blocks are none, nor are positions below 0. */
+enum { ISHZ_KV_BLOCK = 64 };
+enum { ISHZ_KV_INT8 = 0, ISHZ_KV_E4M3 = 1 };
+
+/* Per-head RMS norm, y = x / sqrt(mean x^2 + eps) * weight [dim] (null weight: none), and rotation of the
+   first `rot` values (a multiple of 16, 0: none) of q's and k's heads, in fp32, rounded once. Pairs are
+   (i, i + rot/2), or (2i, 2i + 1) when interleaved. turns [rot/2]: turns a position of each pair,
+   inv_freq / (2 pi), as a fraction of 2^64, so that the angle is exact at any position; factor multiplies
+   both cosine and sine. Outputs [rows][heads][dim], contiguous, may be the inputs where those are too.
+   q_heads or k_heads may be 0. */
+int ishz_norm_rope(const void *q, int64_t q_row, int64_t q_head, int q_heads, const void *k, int64_t k_row,
+                   int64_t k_head, int k_heads, int dtype, int rows, int dim, const int32_t *positions,
+                   const uint64_t *turns, int rot, int interleaved, float factor, const float *q_weight,
+                   const float *k_weight, float eps, void *q_out, void *k_out, ishz_stream_t stream);
+
+/* The call's keys and values into the cache, keys normed and rotated first as in ishz_norm_rope (k_weight
+   null and rot 0: as they are), and q's heads with them into q_out (q_heads 0: none), in one launch.
+   A block that starts with this call's tokens gets for each head the scale max|x| / 127 (int8) or
+   max|x| / 448 (e4m3), 2^-126 at least. A partly filled block keeps its scale unless a new token is too large
+   for it, and then grows it by the least power of two that holds it, its older codes rounded to the new
+   scale. Codes are the nearest, ties to even. An infinity or NaN makes the scale of its block and head NaN, until the
+   block is started again. A block that is written belongs to one sequence of the call. max_rows: at least
+   the most rows of a sequence (tokens of blocks beyond it are not written). */
+int ishz_kv_append(const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head,
+                   int dtype, int rows, void *k_codes, void *v_codes, float *k_scale, float *v_scale, int format,
+                   int blocks, int heads, int dim, const int32_t *table, int width, const int32_t *lengths,
+                   const int32_t *starts, int sequences, int max_rows, const void *q, int64_t q_row,
+                   int64_t q_head, int q_heads, const int32_t *positions, const uint64_t *turns, int rot,
+                   int interleaved, float factor, const float *q_weight, const float *k_weight, float eps,
+                   void *q_out, ishz_stream_t stream);
+
+/* The last `tail` tokens of each sequence: k_out and v_out [sequences][tail][heads][dim] in dtype, zeros
+   where a sequence has fewer. */
+int ishz_kv_read(const void *k_codes, const void *v_codes, const float *k_scale, const float *v_scale, int format,
+                 int blocks, int heads, int dim, const int32_t *table, int width, const int32_t *lengths,
+                 int sequences, int tail, int dtype, void *k_out, void *v_out, ishz_stream_t stream);
+
+/* out [rows][q_heads][dim] = softmax(scale q K^T) V for each of the call's rows, q head h over the cache's head
+   h / (q_heads / heads). causal: a row sees tokens up to its own position; window w > 0 (causal calls): the last
+   w of those. Not causal: all its sequence's tokens. A row that sees no token gives zeros; rows of no sequence are
+   left alone. max_rows and max_length: at least the most rows and tokens of a sequence, from which the work is
+   divided; rows beyond max_rows are left alone. workspace: ishz_kv_attend_workspace_size bytes (may be 0),
+   16-byte aligned. Sums are in a fixed order: the same call gives the same bits. */
+size_t ishz_kv_attend_workspace_size(int rows, int q_heads, int heads, int dim, int sequences, int max_rows,
+                                     int max_length);
+int ishz_kv_attend(const void *q, int64_t q_row, int64_t q_head, int q_heads, int dtype, int rows,
+                   const void *k_codes, const void *v_codes, const float *k_scale, const float *v_scale, int format,
+                   int blocks, int heads, int dim, const int32_t *table, int width, const int32_t *lengths,
+                   const int32_t *starts, int sequences, int max_rows, int max_length, float scale, int causal,
+                   int window, void *out, void *workspace, size_t workspace_bytes, ishz_stream_t stream);
+
 /* ---------------------------------------------------------------- GGUF container (host side)
  * GGUFFile (Config/GGUFFile.swift:179-397): header, metadata and tensor table of a .gguf file,
  * the tensor bytes left in a read-only memory mapping. Malformed or unsupported files give

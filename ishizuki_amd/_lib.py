@@ -14,6 +14,9 @@ OK, DECLINED, EINVAL, EHIP = 0, 1, 2, 3
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 
 P, I, U32, SZ, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint32, ctypes.c_size_t, ctypes.c_float
+L64 = ctypes.c_int64
+_POOL = [P, P, P, P, I, I, I, I]        # a cache: codes, scales, format, blocks, heads, dim
+_TURN = [P, P, I, I, F, P, P, F]        # positions, turns, rot, interleaved, factor, norm weights, eps
 _SIGS = {
     "ishz_last_error": (ctypes.c_char_p, []),
     "ishz_version": (I, []),
@@ -47,6 +50,11 @@ _SIGS = {
     "ishz_moe_swiglu": (I, [U32, P, I, I, I, P, I, I, I, P, P, P, SZ, I, P, P, P, P, P, P, SZ, P]),
     "ishz_moe_swiglu_affine": (I, [P, I, I, I, P, I, I, I, P, P, P, P, P, P, P, P, P, I, I, I, I, P, P, P, P, P, P, SZ,
                                    P]),
+    "ishz_norm_rope": (I, [P, L64, L64, I, P, L64, L64, I, I, I, I, *_TURN, P, P, P]),
+    "ishz_kv_append": (I, [P, L64, L64, P, L64, L64, I, I, *_POOL, P, I, P, P, I, I, P, L64, L64, I, *_TURN, P, P]),
+    "ishz_kv_read": (I, [*_POOL, P, I, P, I, I, I, P, P, P]),
+    "ishz_kv_attend_workspace_size": (SZ, [I, I, I, I, I, I, I]),
+    "ishz_kv_attend": (I, [P, L64, L64, I, I, I, *_POOL, P, I, P, P, I, I, I, F, I, I, P, P, SZ, P]),
     "ishz_ggml_type_known": (I, [U32]),
     "ishz_ggml_geometry": (I, [U32, ctypes.POINTER(I), ctypes.POINTER(I)]),
     "ishz_gguf_open": (I, [ctypes.c_char_p, ctypes.POINTER(P)]),

@@ -1,0 +1,186 @@
+// What the attention kernels share: the 8-bit cache's geometry and codes, the call's rows, per-head
+// norms and the position rotation.
+#pragma once
+#include "common.h"
+
+namespace attn {
+constexpr int BLOCK = ISHZ_KV_BLOCK;  // tokens that share a scale, for each head
+
+// The pool: codes of keys [blocks][heads][64][dim] and of values [blocks][heads][dim][64], their scales
+// [blocks][heads]. Values stand with their tokens contiguous because P V contracts over tokens: a lane's
+// 16-byte load is then a whole matrix operand, and neither keys nor values pass through LDS to be turned.
+struct Pool {
+  uint8_t *k, *v;
+  float *ks, *vs;
+  int blocks, heads, dim;
+  // Offsets pass 32 bits in a long cache (64 heads * dim 128 * 64 tokens * 2^13 blocks = 2^32).
+  DEV size_t tile(int block, int head) const { return ((size_t)block * heads + head) * (BLOCK * dim); }
+  DEV size_t scale(int block, int head) const { return (size_t)block * heads + head; }
+};
+
+// The call's rows: sequence s has rows starts[s]..starts[s+1] of `rows` and lengths[s] tokens in the cache,
+// those rows' own among them; its blocks are table[s * width ...].
+struct Rows {
+  const int32_t *table, *lengths, *starts;
+  int sequences, width, rows;
+  DEV int first(int s) const { return min(max(starts[s], 0), rows); }
+  DEV int count(int s) const { return max(min(starts[s + 1], rows) - first(s), 0); }
+  DEV int length(int s) const { return max(min(lengths[s], width * BLOCK), 0); }
+  // The block that holds tokens 64 j.. of s, or -1: an entry outside the pool holds no tokens.
+  DEV int block(int s, int j, int blocks) const {
+    if (j < 0 || j >= width) return -1;
+    const int b = table[(size_t)s * width + j];
+    return b >= 0 && b < blocks ? b : -1;
+  }
+};
+
+// ---------------------------------------------------------------- codes
+template <int FMT>
+constexpr float LIMIT = FMT == ISHZ_KV_INT8 ? 127.0f : 448.0f;
+
+// Four codes as exact fp16 values. int8: offset by 128, each byte under the exponent byte of 1024 (0x64),
+// minus 1152: one xor, two byte permutes, two packed subtractions. e4m3: two conversions of two.
+template <int FMT>
+DEV u2 decode4(uint32_t c) {
+  if (FMT == ISHZ_KV_INT8) {
+    c ^= 0x80808080u;
+    const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    return u2{as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, c, 0x04010400u)) - off),
+              as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, c, 0x04030402u)) - off)};
+  }
+  return u2{as_u32(__builtin_bit_cast(h2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, false))),
+            as_u32(__builtin_bit_cast(h2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, true)))};
+}
+template <int FMT>
+DEV h8 decode8(uint32_t lo, uint32_t hi) {
+  const u2 a = decode4<FMT>(lo), b = decode4<FMT>(hi);
+  return as_h8(u4{a.x, a.y, b.x, b.y});
+}
+// Four codes as fp32 values.
+template <int FMT>
+DEV f4 decode4f(uint32_t c) {
+  if (FMT == ISHZ_KV_INT8)
+    return f4{(float)(int8_t)c, (float)(int8_t)(c >> 8), (float)(int8_t)(c >> 16), (float)((int32_t)c >> 24)};
+  return f4{__builtin_amdgcn_cvt_f32_fp8(c, 0), __builtin_amdgcn_cvt_f32_fp8(c, 1), __builtin_amdgcn_cvt_f32_fp8(c, 2),
+            __builtin_amdgcn_cvt_f32_fp8(c, 3)};
+}
+// Four values, in units of the scale, as codes: the nearest, ties to even.
+template <int FMT>
+DEV uint32_t encode4(float a, float b, float c, float d) {
+  const float m = LIMIT<FMT>;
+  a = fminf(fmaxf(a, -m), m), b = fminf(fmaxf(b, -m), m), c = fminf(fmaxf(c, -m), m), d = fminf(fmaxf(d, -m), m);
+  if (FMT == ISHZ_KV_INT8)
+    return ((uint32_t)(int)rintf(a) & 255) | ((uint32_t)(int)rintf(b) & 255) << 8 | ((uint32_t)(int)rintf(c) & 255) << 16 |
+           (uint32_t)(int)rintf(d) << 24;
+  uint32_t r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+
+// ---------------------------------------------------------------- activations, eight at a time
+template <int DT>
+DEV void load8(const void *p, size_t i, float *o) {
+  if (DT == ISHZ_DT_F32) {
+    const f4 a = *(const f4 *)((const float *)p + i), b = *(const f4 *)((const float *)p + i + 4);
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] = a[j], o[4 + j] = b[j];
+  } else {
+    const u4 v = *(const u4 *)((const uint16_t *)p + i);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      o[2 * j] = DT == ISHZ_DT_F16 ? h2f(v[j] & 0xffff) : __builtin_bit_cast(float, v[j] << 16);
+      o[2 * j + 1] = DT == ISHZ_DT_F16 ? h2f(v[j] >> 16) : __builtin_bit_cast(float, v[j] & 0xffff0000u);
+    }
+  }
+}
+template <int DT>
+DEV uint32_t narrow2(float a, float b) {
+  if (DT == ISHZ_DT_F16) return (uint32_t)f2h(a) | (uint32_t)f2h(b) << 16;
+  return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16;
+}
+template <int DT>
+DEV void store8(void *p, size_t i, const float *v) {
+  if (DT == ISHZ_DT_F32) {
+    *(f4 *)((float *)p + i) = f4{v[0], v[1], v[2], v[3]};
+    *(f4 *)((float *)p + i + 4) = f4{v[4], v[5], v[6], v[7]};
+  } else {
+    *(u4 *)((uint16_t *)p + i) = u4{narrow2<DT>(v[0], v[1]), narrow2<DT>(v[2], v[3]), narrow2<DT>(v[4], v[5]),
+                                   narrow2<DT>(v[6], v[7])};
+  }
+}
+
+// ---------------------------------------------------------------- norm and rotation of a head
+// y = x * rsqrt(mean x^2 + eps) * w over the head, then the first `rot` values turned in pairs by their
+// position's angle: (a, b) -> (a cos - b sin, b cos + a sin), pairs (i, i + rot/2) or, interleaved, (2i, 2i+1).
+struct Turn {
+  const int32_t *positions;
+  const uint64_t *turns;  // [rot/2] turns a position, as fractions of 2^64
+  int rot, interleaved;
+  float factor;  // on both cosine and sine
+};
+
+// A lane holds two chunks of eight values of a head, chosen so that both values of every pair are its own:
+// unit u of dim/16. Returns the chunks' first values.
+DEV void unit_chunks(int u, int rot, bool interleaved, int *a, int *b) {
+  if (interleaved || u >= rot / 16) *a = 16 * u, *b = 16 * u + 8;
+  else *a = 8 * u, *b = rot / 2 + 8 * u;
+}
+
+// cos and sin of `phase` turns / 2^32. The angle never leaves the integers until it is within an eighth of a turn
+// of a multiple of a quarter: a position's phase is the low 64 bits of position * turns, exact for any int32
+// position, where an fp32 angle of position 10^6 is off by 0.06. Taylor series to 2^-25 on [-pi/4, pi/4].
+DEV void cos_sin(uint32_t phase, float *c, float *s) {
+  const uint32_t quarter = (phase + 0x20000000u) >> 30;
+  const float t = (float)(int32_t)(phase - (quarter << 30)) * 1.46291807926715968e-9f;  // 2 pi / 2^32
+  const float z = t * t;
+  const float sn = t + t * z * (-1.0f / 6 + z * (1.0f / 120 + z * (-1.0f / 5040 + z * (1.0f / 362880))));
+  const float cs = 1.0f + z * (-0.5f + z * (1.0f / 24 + z * (-1.0f / 720 + z * (1.0f / 40320 - z * (1.0f / 3628800)))));
+  const float x = quarter & 1 ? sn : cs, y = quarter & 1 ? cs : sn;
+  *c = (quarter + 1) & 2 ? -x : x;
+  *s = quarter & 2 ? -y : y;
+}
+DEV uint32_t phase_of(uint64_t turns, int32_t position) {
+  return (uint32_t)(((uint64_t)(int64_t)position * turns) >> 32);
+}
+// The eight angles of unit u (u < rot / 16).
+DEV void unit_angles(const Turn &t, int u, int32_t position, float *c, float *s) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    cos_sin(phase_of(t.turns[8 * u + i], position), c + i, s + i);
+    c[i] *= t.factor, s[i] *= t.factor;
+  }
+}
+// x: the unit's sixteen values, in place.
+DEV void unit_turn(bool interleaved, const float *c, const float *s, float *x) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const float a = interleaved ? x[2 * i] : x[i], b = interleaved ? x[2 * i + 1] : x[8 + i];
+    const float p = a * c[i] - b * s[i], q = b * c[i] + a * s[i];
+    if (interleaved) x[2 * i] = p, x[2 * i + 1] = q;
+    else x[i] = p, x[8 + i] = q;
+  }
+}
+// Sum over the head's U = dim / 16 lanes (4, 8 or 16).
+template <int U>
+DEV float head_sum(float v) {
+  v += ISHZ_DPP(v, 0xB1);
+  v += ISHZ_DPP(v, 0x4E);
+  if (U >= 8) v += ISHZ_DPP(v, 0x141);
+  if (U >= 16) v += ISHZ_DPP(v, 0x140);
+  return v;
+}
+// Norms the unit's sixteen values in place; every lane of the head calls it. w: the head's weight.
+template <int U>
+DEV void unit_norm(float *x, const float *w, int ca, int cb, float eps) {
+  float sum = 0;
+#pragma unroll
+  for (int i = 0; i < 16; i++) sum += x[i] * x[i];
+  const float r = 1.0f / sqrtf(head_sum<U>(sum) * (1.0f / (16 * U)) + eps);
+#pragma unroll
+  for (int i = 0; i < 16; i++) x[i] *= r * w[i < 8 ? ca + i : cb + i - 8];
+}
+
+// What every call on the cache refuses (attn_cache.hip).
+int check_pool(const void *k, const void *v, const float *ks, const float *vs, int format, int blocks, int heads, int dim);
+int check_rows(const int32_t *table, const int32_t *lengths, const int32_t *starts, int sequences, int width, int rows);
+int check_heads(const void *x, int dtype, int64_t row, int64_t head, const void *out);
+}  // namespace attn

@@ -1,0 +1,522 @@
+"""Attention over the 8-bit cache on the GPU, against plain implementations in 64 bits.
+
+Tolerances count roundings: u(t) = finfo(t).eps / 2 is half a step of a type, relative to the value.
+"""
+import math
+
+import pytest
+import torch
+
+from ishizuki_amd import attention
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+LIMIT = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+INT8, E4M3 = torch.int8, torch.float8_e4m3fn
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def normal(seed, *shape, dtype=F32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def i32(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def make_batch(lengths, rows, blocks=None, width=None, seed=0, spare=2):
+    """(batch on the GPU, blocks in the pool): sequences of the given tokens and new rows, blocks in a random order."""
+    need = [-(-n // 64) for n in lengths]
+    blocks = sum(need) + spare if blocks is None else blocks
+    order = torch.randperm(blocks, generator=torch.Generator().manual_seed(seed)).tolist()
+    width = max(max(need), 1) if width is None else width
+    table = torch.full((len(lengths), width), -1, dtype=torch.int32)
+    at = 0
+    for s, n in enumerate(need):
+        table[s, :n] = torch.tensor(order[at:at + n], dtype=torch.int32)
+        at += n
+    starts = i32(0, *torch.tensor(rows).cumsum(0).tolist())
+    return attention.Batch(table.to(DEV), i32(*lengths).to(DEV), starts.to(DEV), max(rows), max(lengths)), blocks
+
+
+def random_cache(blocks, heads, dim, dtype, seed=0):
+    """A pool of finite codes and scales of about a unit value."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((2, blocks, heads, 64 * dim), generator=g)
+    scale = x.abs().amax(-1) / LIMIT[dtype]
+    x = x / scale[..., None]
+    codes = (x.round() if dtype is INT8 else x).to(dtype).view(INT8)
+    c = attention.new_cache(blocks, heads, dim, dtype, device="cpu")
+    c.k.view(INT8).copy_(codes[0].view(c.k.shape))
+    c.v.view(INT8).copy_(codes[1].view(c.v.shape))
+    return attention.Cache(c.k, c.v, scale[0].contiguous(), scale[1].contiguous())
+
+
+def gpu(cache):
+    return attention.Cache(*(t.to(DEV) for t in cache))
+
+
+def values(cache, batch, s, length=None):
+    """(k, v) [tokens, heads, dim] of sequence s in 64 bits, NaN where the table has no block."""
+    length = int(batch.lengths[s]) if length is None else length
+    blocks, heads, _, dim = cache.k.shape
+    k = torch.full((length, heads, dim), float("nan"), dtype=torch.float64)
+    v = k.clone()
+    for j in range(-(-length // 64)):
+        b = int(batch.table[s, j]) if j < batch.table.shape[1] else -1
+        if not 0 <= b < blocks:
+            continue
+        n = min(64, length - 64 * j)
+        k[64 * j:64 * j + n] = (cache.k[b].cpu().double() * cache.k_scale[b].cpu().double()[:, None, None])[:, :n].transpose(0, 1)
+        v[64 * j:64 * j + n] = (cache.v[b].cpu().double() * cache.v_scale[b].cpu().double()[:, None, None])[:, :, :n].permute(2, 0, 1)
+    return k, v
+
+
+# ---------------------------------------------------------------- norms and rotation
+def rope_reference(x, positions, inv_freq, weight, eps, interleaved, factor=1.0):
+    """[rows, heads, dim] in 64 bits."""
+    x = x.double()
+    if weight is not None:
+        x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * weight.double()
+    rot = 2 * len(inv_freq)
+    if rot == 0:
+        return x
+    angle = positions.double()[:, None, None] * torch.tensor(inv_freq, dtype=torch.float64)
+    c, s = angle.cos() * factor, angle.sin() * factor
+    a, b = (x[..., 0:rot:2], x[..., 1:rot:2]) if interleaved else (x[..., :rot // 2], x[..., rot // 2:rot])
+    y = x.clone()
+    if interleaved:
+        y[..., 0:rot:2], y[..., 1:rot:2] = a * c - b * s, b * c + a * s
+    else:
+        y[..., :rot // 2], y[..., rot // 2:rot] = a * c - b * s, b * c + a * s
+    return y
+
+
+def rope_tolerance(y, x, weight, eps, dtype, factor=1.0):
+    """Half a step of the output, and in fp32: the norm's sum of squares, root, quotient and two products (8 half steps;
+    the sum's tree adds at most 8 more), the angle's cosine and sine (half a step of the phase's 2^-25 turns, 2 pi 2^-26,
+    and 3 half steps of the series: 2^-23 in all), two products and a sum (3): below 2^-19 of the pair's size."""
+    x = x.double()
+    if weight is not None:
+        x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * weight.double()
+    size = x.abs().amax(-1, keepdim=True) * math.sqrt(2) * factor
+    return u(dtype) * y.abs() + 2.0 ** -19 * size + (2.0 ** -25 if dtype is F16 else 1e-38)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim,rot,interleaved", [(64, 64, False), (128, 128, False), (256, 64, True), (128, 32, False),
+                                                 (256, 256, False), (64, 16, True), (128, 0, False)])
+@pytest.mark.parametrize("rows,heads,kv", [(1, 5, 1), (7, 32, 8), (2049, 3, 2)])
+def test_norm_rope(dtype, dim, rot, interleaved, rows, heads, kv):
+    print(f"norm_rope {dtype} {rows} x ({heads}, {kv}) x {dim} rot {rot}", flush=True)
+    qkv = normal(1, rows, heads + 2 * kv, dim, dtype=dtype)
+    positions = torch.arange(rows, dtype=torch.int32) * 977 + 1000003
+    inv = [1e6 ** (-2.0 * i / max(rot, 1)) for i in range(rot // 2)]
+    wq, wk = 1 + normal(2, dim) / 4, 1 + normal(3, dim) / 4
+    d = qkv.to(DEV)
+    table = attention.turns(inv_freq=inv, device=DEV) if rot else None
+    q, k = attention.norm_rope(d[:, :heads], d[:, heads:heads + kv], positions.to(DEV), table, wq.to(DEV), wk.to(DEV),
+                               eps=1e-5, interleaved=interleaved, factor=1.25)
+    for got, x, w in ((q, qkv[:, :heads], wq), (k, qkv[:, heads:heads + kv], wk)):
+        y = rope_reference(x, positions, inv, w, 1e-5, interleaved, 1.25)
+        assert torch.all((got.cpu().double() - y).abs() <= rope_tolerance(y, x, w, 1e-5, dtype, 1.25))
+
+
+def test_norm_rope_parts():
+    """No weight: no norm; no turns: no rotation; negative and far positions; a row of zeros; in place through the C call's
+    own rules; k heads alone."""
+    x = normal(4, 5, 2, 128, dtype=F16)
+    x[3] = 0
+    d, positions = x.to(DEV), i32(-3, 0, 5, 7, 2 ** 31 - 1)
+    inv = [1e4 ** (-2.0 * i / 128) for i in range(64)]
+    q, k = attention.norm_rope(d, d)
+    assert torch.equal(q, d) and torch.equal(k, d)
+    q, k = attention.norm_rope(d, d[:, :1], positions.to(DEV), attention.turns(inv_freq=inv, device=DEV))
+    y = rope_reference(x, positions, inv, None, 0, False)
+    assert torch.all((q.cpu().double() - y).abs() <= rope_tolerance(y, x, None, 0, F16) + 2.0 ** -20 * x.double().abs().amax())
+    assert torch.equal(k, q[:, :1]) and torch.all(q[3] == 0)
+    w = torch.full((128,), 2.0, device=DEV)
+    q, k = attention.norm_rope(d[:, :0], d, k_weight=w)
+    y = rope_reference(x, positions, [], w.cpu(), 1e-6, False)
+    assert q.shape == (5, 0, 128)
+    assert torch.all((k.cpu().double() - y).abs() <= rope_tolerance(y, x, w.cpu(), 1e-6, F16))
+
+
+# ---------------------------------------------------------------- writing and reading
+class Model:
+    """The cache in 64 bits on the CPU: codes [blocks, heads, 64, dim] as numbers, scales; appends as the header says."""
+
+    def __init__(self, cache):
+        self.dtype = cache.k.dtype
+        self.held = [cache.k.cpu().double(), cache.v.cpu().double().transpose(-1, -2).contiguous()]
+        self.scale = [cache.k_scale.cpu().double(), cache.v_scale.cpu().double()]
+        self.ratio = [torch.full_like(x, math.nan) for x in self.held]  # of what was coded since the last check
+
+    def code(self, x):
+        m = LIMIT[self.dtype]
+        x = x.clamp(-m, m)
+        if self.dtype is INT8:
+            return x.round()
+        step = 2.0 ** (torch.floor(torch.log2(x.abs().clamp(min=2.0 ** -6))) - 3)
+        return (x / step).round() * step
+
+    def append(self, which, new, table, first):
+        """new [rows, heads, dim] at positions first.. of the sequence whose blocks `table` lists."""
+        for j in sorted({(first + i) // 64 for i in range(new.shape[0]) if first + i >= 0}):
+            b = table[j] if j < len(table) else -1
+            if not 0 <= b < self.held[0].shape[0]:
+                continue
+            rows = [i for i in range(new.shape[0]) if (first + i) // 64 == j and first + i >= 0]
+            slots = [(first + i) % 64 for i in rows]
+            x = new[rows].double()
+            for h in range(x.shape[1]):
+                amax = float(x[:, h].abs().max()) if torch.isfinite(x[:, h]).all() else math.nan
+                s = float(self.scale[which][b, h])
+                if math.isnan(amax):
+                    s = math.nan
+                elif slots[0] == 0:
+                    s = max(amax / LIMIT[self.dtype], 2.0 ** -126)
+                else:
+                    s = max(s, 2.0 ** -126) if s == s else s
+                    k = 0
+                    while amax > LIMIT[self.dtype] * s * 2.0 ** k * (1 + 2.0 ** -22):
+                        k += 1
+                    s *= 2.0 ** k
+                    if k:
+                        self.held[which][b, h, :slots[0]] = self.code(self.held[which][b, h, :slots[0]] / 2.0 ** k)
+                self.scale[which][b, h] = s
+                self.ratio[which][b, h, slots] = x[:, h] / s
+                self.held[which][b, h, slots] = 0.0 if math.isnan(s) else self.code(x[:, h] / s)
+
+    def check(self, cache, key_error=0.0):
+        """Scales to two half steps of fp32 (a quotient), codes equal but where x / s lies within fp32's roundings of the
+        border between two neighbours (a quotient or a reciprocal and a product: four half steps); keys that were computed
+        may be off by `key_error` of their head's largest before they are coded. Then goes on from what the GPU holds."""
+        got = [cache.k.cpu().double(), cache.v.cpu().double().transpose(-1, -2).contiguous()]
+        for which, scale in enumerate((cache.k_scale, cache.v_scale)):
+            a, b = scale.cpu().double(), self.scale[which]
+            off = 0.0 if which else key_error
+            assert torch.equal(a.isnan(), b.isnan())
+            assert torch.all(((a - b).abs() <= (2 * u(F32) + off) * b)[~b.isnan()])
+            x, y, ratio = got[which], self.held[which], self.ratio[which]
+            differ = x != y
+            near = (ratio - (x + y) / 2).abs() <= 4 * u(F32) * ratio.abs() + 2 * off * LIMIT[self.dtype]
+            assert torch.all(near[differ]), float(differ.double().mean())
+            step = 1.0 if self.dtype is INT8 else 2.0 ** (torch.floor(torch.log2(torch.minimum(x.abs(), y.abs()).clamp(min=2.0 ** -6))) - 3)
+            assert torch.all((x - y).abs() <= step)
+            self.held[which], self.scale[which] = x, a
+            self.ratio[which] = torch.full_like(x, math.nan)
+
+
+@pytest.mark.parametrize("dtype", [INT8, E4M3])
+@pytest.mark.parametrize("x", [F16, BF16, F32])
+@pytest.mark.parametrize("heads,dim", [(3, 64), (8, 128), (1, 256)])
+def test_append_and_read(dtype, x, heads, dim):
+    """Ragged sequences written in several calls: fresh and partly filled blocks, one token and many, scales that grow."""
+    print(f"append {dtype} {x} {heads} x {dim}", flush=True)
+    calls = [[63, 0, 130, 1], [1, 0, 1, 70], [1, 5, 64, 1], [200, 1, 1, 0]]
+    total = [sum(c[s] for c in calls) for s in range(4)]
+    whole, blocks = make_batch(total, [0] * 4, seed=dim)
+    cache = random_cache(blocks, heads, dim, dtype, seed=7)
+    model, cache = Model(cache), gpu(cache)
+    held = [0] * 4
+    for n, rows in enumerate(calls):
+        size = 3.0 ** n  # later tokens are larger
+        k, v = (normal(10 * n + i, sum(rows), heads, dim) * size for i in (1, 2))
+        k[:, :, ::17] *= 6
+        k, v = k.to(x), v.to(x)
+        starts = [0, *torch.tensor(rows).cumsum(0).tolist()]
+        held = [h + r for h, r in zip(held, rows)]
+        batch = whole._replace(lengths=i32(*held).to(DEV), starts=i32(*starts).to(DEV), max_rows=max(rows))
+        assert attention.append(k.to(DEV), v.to(DEV), cache, batch) is True
+        for s in range(4):
+            for which, t in enumerate((k, v)):
+                model.append(which, t[starts[s]:starts[s + 1]], whole.table[s].tolist(), held[s] - rows[s])
+        model.check(cache)
+    for out in (F16, BF16, F32):
+        for tail in (1, 63, 64, 65, max(held) + 9):
+            got = attention.read(cache, batch, tail=tail, dtype=out)
+            for s in range(4):
+                for y, ref in zip(got, values(cache, batch, s)):
+                    y, ref = y[s].cpu(), ref[-tail:]
+                    assert torch.all(y[:tail - ref.shape[0]] == 0)
+                    y = y[tail - ref.shape[0]:].double()
+                    # a product of 24 and 8 bits rounded to fp32 and then to the output
+                    assert torch.all((y - ref).abs() <= (u(out) + u(F32)) * ref.abs() + (2.0 ** -25 if out is F16 else 0))
+
+
+@pytest.mark.parametrize("dtype", [INT8, E4M3])
+@pytest.mark.parametrize("dim,rot,interleaved", [(128, 128, False), (64, 32, True), (256, 64, False)])
+def test_append_with_norms_and_rotation(dtype, dim, rot, interleaved):
+    rows, lengths, heads, kv = [1, 90, 0, 3], [40, 90, 0, 130], 6, 2
+    batch, blocks = make_batch(lengths, rows, seed=3)
+    cache = random_cache(blocks, kv, dim, dtype, seed=8)
+    model, cache = Model(cache), gpu(cache)
+    qkv = normal(5, sum(rows), heads + 2 * kv, dim, dtype=BF16)
+    positions = torch.cat([torch.arange(n - r, n) for n, r in zip(lengths, rows)]).int() + 500000
+    inv = [1e4 ** (-2.0 * i / rot) for i in range(rot // 2)]
+    wq, wk = 1 + normal(2, dim) / 4, 2 + normal(3, dim) / 4
+    d = qkv.to(DEV)
+    q = attention.append(d[:, heads:heads + kv], d[:, heads + kv:], cache, batch, q=d[:, :heads],
+                         positions=positions.to(DEV), turns=attention.turns(inv_freq=inv, device=DEV), q_weight=wq.to(DEV),
+                         k_weight=wk.to(DEV), interleaved=interleaved)
+    y = rope_reference(qkv[:, :heads], positions, inv, wq, 1e-6, interleaved)
+    assert torch.all((q.cpu().double() - y).abs() <= rope_tolerance(y, qkv[:, :heads], wq, 1e-6, BF16))
+    k = rope_reference(qkv[:, heads:heads + kv], positions, inv, wk, 1e-6, interleaved)
+    at = 0
+    for s, r in enumerate(rows):
+        for which, t in enumerate((k, qkv[:, heads + kv:])):
+            model.append(which, t[at:at + r], batch.table[s].tolist(), lengths[s] - r)
+        at += r
+    model.check(cache, key_error=2.0 ** -18)  # see rope_tolerance: 2^-19 sqrt 2 of the head's largest
+
+
+def test_append_again_changes_nothing():
+    batch, blocks = make_batch([70, 3], [7, 2])
+    cache = gpu(random_cache(blocks, 2, 128, INT8, seed=9))
+    k, v = normal(1, 9, 2, 128).to(DEV) * 20, normal(2, 9, 2, 128).to(DEV)
+    attention.append(k, v, cache, batch)
+    once = [t.clone() for t in cache]
+    attention.append(k, v, cache, batch)
+    assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(once, cache))
+
+
+@pytest.mark.parametrize("dtype", [INT8, E4M3])
+def test_append_of_what_is_not_a_number(dtype):
+    """An infinity or NaN shows as NaN in its block and head alone; zeros and the smallest values are codes of 0."""
+    batch, blocks = make_batch([128, 64], [128, 64])
+    cache = gpu(random_cache(blocks, 3, 64, dtype))
+    k, v = normal(1, 192, 3, 64), normal(2, 192, 3, 64)
+    k[5, 1, 7], v[70, 2, 0] = math.inf, math.nan
+    k[128:, 0] = 0
+    v[128:, 1] = 1e-45
+    attention.append(k.to(DEV), v.to(DEV), cache, batch)
+    gk, gv = attention.read(cache, batch, dtype=F32)
+    bad_k, bad_v = torch.zeros(2, 128, 3, 64, dtype=torch.bool), torch.zeros(2, 128, 3, 64, dtype=torch.bool)
+    bad_k[0, :64, 1], bad_v[0, 64:, 2] = True, True
+    assert torch.equal(gk.cpu().isnan(), bad_k) and torch.equal(gv.cpu().isnan(), bad_v)
+    assert torch.all(gk[1, :, 0] == 0) and torch.all(gv[1, :, 1] == 0)
+    attention.append(k[128:].to(DEV), v[128:].to(DEV), cache, batch._replace(starts=i32(0, 64, 64).to(DEV), lengths=i32(64, 0).to(DEV)))
+    assert torch.isfinite(cache.k_scale[batch.table[0, 0].item()]).all()  # started again
+
+
+def test_append_leaves_the_rest_alone():
+    """Holes of the table, tokens past it, rows past max_rows' blocks and other blocks stay as they were."""
+    table = i32(2, -1, 99, 5).view(1, 4).to(DEV)
+    batch = attention.Batch(table, i32(300).to(DEV), i32(0, 290).to(DEV), 290, 300)
+    cache = gpu(random_cache(8, 2, 64, INT8))
+    before = attention.Cache(*(t.clone() for t in cache))
+    model = Model(cache)
+    k, v = normal(1, 290, 2, 64), normal(2, 290, 2, 64)
+    attention.append(k.to(DEV), v.to(DEV), cache, batch)
+    # 300 tokens are cut at the table's 256: the rows are then the last 290 of those, the first 34 of them nowhere
+    for which, t in enumerate((k, v)):
+        model.append(which, t, [2, -1, 99, 5], 256 - 290)
+    model.check(cache)
+    for b in (0, 1, 3, 4, 6, 7):
+        assert torch.equal(cache.k[b], before.k[b]) and torch.equal(cache.v[b], before.v[b])
+
+
+# ---------------------------------------------------------------- attention
+def attention_reference(q, cache, batch, scale, causal, window):
+    """(out, bound) [rows, heads, dim] in 64 bits: bound is sum of weights |v|, and what the logits' roundings move."""
+    blocks, heads, _, dim = cache.k.shape
+    group = q.shape[1] // heads
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    bound, shift = torch.zeros_like(out), torch.zeros(q.shape[0], q.shape[1], 1, dtype=torch.float64)
+    starts = batch.starts.tolist()
+    for s in range(len(starts) - 1):
+        n, length = starts[s + 1] - starts[s], min(int(batch.lengths[s]), 64 * batch.table.shape[1])
+        k, v = values(cache, batch, s, length)
+        hole = torch.tensor([not 0 <= int(batch.table[s, t // 64]) < blocks for t in range(length)], dtype=torch.bool)
+        k[hole], v[hole] = 0, 0
+        token = torch.arange(length)
+        for i in range(n):
+            at = length - n + i
+            seen = ~hole
+            if causal:
+                seen = seen & (token <= at)
+                if window:
+                    seen = seen & (token > at - window)
+            if not seen.any():
+                continue
+            for h in range(heads):
+                x = q[starts[s] + i, h * group:(h + 1) * group].double()
+                logit = x @ k[seen, h].T * scale
+                w = torch.softmax(logit, -1)
+                out[starts[s] + i, h * group:(h + 1) * group] = w @ v[seen, h]
+                bound[starts[s] + i, h * group:(h + 1) * group] = w @ v[seen, h].abs()
+                shift[starts[s] + i, h * group:(h + 1) * group, 0] = (x.abs() @ k[seen, h].abs().T * scale).amax(-1)
+    return out, bound, shift
+
+
+def attention_close(got, q, ref):
+    """Half a step of the output's type; of each weight half a step of fp16 (2^-11), exp2 and the sums in fp32 (2^-20 in
+    all), weights below fp16's normals 2^-25 of the largest each; a logit's sum of dim products and three scalings, and q's
+    fp16 image (2^-25 of a row's largest a value): dim + 8 half steps of the products' sizes, twice (numerator and sum)."""
+    out, bound, shift = ref
+    dim = q.shape[-1]
+    tol = u(got.dtype) * out.abs() + (2.0 ** -11 + 2.0 ** -20 + 2 * (dim + 8) * u(F32) * shift) * bound
+    tol = tol + 2.0 ** -25 * bound.amax() * 64 + (2.0 ** -25 if got.dtype is F16 else 0)
+    d = (got.cpu().double() - out).abs()
+    assert torch.all(d <= tol), float((d / tol).max())
+
+
+CASES = [  # lengths, rows, causal, window
+    ([1], [1], True, 0), ([64], [1], True, 0), ([65], [1], True, 0), ([777], [1], True, 0), ([5000], [1], True, 0),
+    ([0, 130, 63, 64], [0, 1, 1, 1], True, 0), ([200, 77], [5, 3], True, 0), ([129, 64], [129, 64], True, 0),
+    ([300], [41], True, 100), ([1000, 70, 9], [2, 70, 1], True, 33), ([513], [3], True, 1), ([200, 1, 0], [7, 33, 0], False, 0),
+    ([20], [37], True, 0), ([150], [150], True, 64),
+]
+
+
+@pytest.mark.parametrize("lengths,rows,causal,window", CASES)
+@pytest.mark.parametrize("heads,group,dim,dtype,x", [(2, 4, 128, INT8, BF16), (1, 1, 64, E4M3, F16), (3, 5, 64, INT8, F16),
+                                                     (2, 8, 256, E4M3, BF16), (1, 16, 128, E4M3, F16), (1, 3, 256, INT8, BF16)])
+def test_attend(lengths, rows, causal, window, heads, group, dim, dtype, x):
+    print(f"attend {lengths} {rows} {causal} {window} {heads} x {group} x {dim} {dtype} {x}", flush=True)
+    batch, blocks = make_batch(lengths, rows, seed=1)
+    cache = random_cache(blocks, heads, dim, dtype, seed=sum(lengths))
+    q = normal(3, sum(rows), heads * group, dim, dtype=x)
+    got = attention.attend(q.to(DEV), gpu(cache), batch, causal=causal, window=window)
+    attention_close(got, q, attention_reference(q, cache, batch, dim ** -0.5, causal, window))
+    again = attention.attend(q.to(DEV), gpu(cache), batch, causal=causal, window=window)
+    assert torch.equal(got, again)
+
+
+def test_attend_sharp_and_large():
+    """Logits of some hundreds: one token takes all the weight, nothing overflows; queries beyond fp16's range."""
+    batch, blocks = make_batch([500], [3], seed=1)
+    cache = random_cache(blocks, 2, 128, INT8, seed=5)
+    q = normal(3, 3, 4, 128) * 3e5
+    q = q.to(BF16)
+    got = attention.attend(q.to(DEV), gpu(cache), batch, scale=1e-3)
+    attention_close(got, q, attention_reference(q, cache, batch, 1e-3, True, 0))
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("dtype", [INT8, E4M3])
+def test_attend_ignores_what_it_does_not_see(dtype, rows):
+    """NaN scales of blocks that no row of a tile sees, or that one row does not; NaN codes and whatever else past the
+    end; holes in the table."""
+    batch, blocks = make_batch([300], [rows], seed=2, width=9)
+    cache = random_cache(blocks, 2, 64, dtype, seed=6)
+    q = normal(3, rows, 4, 64, dtype=F16)
+    batch.table[0, 1], batch.table[0, 2] = -1, blocks + 5
+    ref = attention_reference(q, cache, batch, 0.125, True, 0)
+    last = int(batch.table[0, 4])
+    cache.k.view(INT8)[last, :, 300 - 256:] = 0x7F  # e4m3's NaN
+    cache.v.view(INT8)[last, :, :, 300 - 256:] = 0x7F
+    for b in range(blocks):
+        if b not in batch.table[0].tolist():
+            cache.k_scale[b], cache.v_scale[b] = math.nan, math.inf
+    got = attention.attend(q.to(DEV), gpu(cache), batch)
+    attention_close(got, q, ref)
+    # the last block's scales of no number reach the rows that see it, and no others
+    cache.k_scale[last], cache.v_scale[last] = math.nan, math.nan
+    got = attention.attend(q.to(DEV), gpu(cache), batch).cpu()
+    sees = torch.arange(300 - rows, 300) >= 256
+    assert torch.equal(got.isnan(), sees[:, None, None].expand_as(got))
+    if (~sees).any():
+        keep = tuple(t[~sees] for t in ref)
+        attention_close(got[~sees], q, keep)
+    got = attention.attend(q.to(DEV), gpu(cache), batch, window=5).cpu()
+    first = torch.arange(300 - rows, 300) < 256  # those rows' window lies before the last block
+    assert not got[first].isnan().any()
+
+
+def test_strides_streams_and_rows_of_no_sequence():
+    batch, blocks = make_batch([100, 40], [2, 3], seed=4)
+    cache = random_cache(blocks, 2, 128, INT8, seed=6)
+    wide = normal(3, 9, 11, 128, dtype=F16)
+    q = wide[::1, 1:7]
+    ref = attention_reference(q[:5], cache, batch, 128 ** -0.5, True, 0)
+    c, d = gpu(cache), wide.to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = attention.attend(d[:, 1:7], c, batch)
+    torch.cuda.current_stream().wait_stream(side)
+    attention_close(got[:5], q, ref)
+    half = torch.empty(5, 6, 2, 128, dtype=F16, device=DEV)
+    half[:, :, 0] = d[:5, 1:7]
+    attention_close(attention.attend(half[:, :, 0], c, batch), q, ref)
+
+
+def test_offsets_past_32_bits():
+    """Blocks whose codes lie more than 4 GiB into the pool, written, read and attended to."""
+    heads, dim = 8, 256
+    blocks = (1 << 32) // (heads * 64 * dim) + 6
+    cache = attention.new_cache(blocks, heads, dim, E4M3, device=DEV)
+    table = torch.arange(blocks - 1, blocks - 5, -1, dtype=torch.int32).view(1, 4).to(DEV)
+    k, v = normal(1, 200, heads, dim, dtype=F16), normal(2, 200, heads, dim, dtype=F16)
+    batch = attention.Batch(table, i32(200).to(DEV), i32(0, 200).to(DEV), 200, 200)
+    attention.append(k.to(DEV), v.to(DEV), cache, batch)
+    small = attention.Cache(*(t[-6:].cpu() for t in cache))
+    near = batch._replace(table=table - (blocks - 6))
+    for got, ref in zip(attention.read(cache, batch, dtype=F32), values(small, near, 0)):
+        assert torch.all((got[0].cpu().double() - ref).abs() <= u(F32) * ref.abs())
+    q = normal(3, 1, 8, dim, dtype=F16)
+    one = batch._replace(starts=i32(0, 1).to(DEV), max_rows=1)
+    got = attention.attend(q.to(DEV), cache, one)
+    attention_close(got, q, attention_reference(q, small, near._replace(starts=i32(0, 1)), dim ** -0.5, True, 0))
+
+
+def test_captured_step_follows_the_lengths():
+    """A step (norms, rotation, writing, attention) captured once and replayed as the sequences grow gives what eager
+    calls give, bit for bit."""
+    heads, kv, dim = 8, 2, 128
+    lengths, steps = [60, 127, 1], 6
+    whole, blocks = make_batch([n + steps + 1 for n in lengths], [1, 1, 1], seed=5)
+    first = gpu(random_cache(blocks, kv, dim, INT8, seed=2))
+    table = attention.turns(dim, device=DEV)
+    w = torch.ones(dim, device=DEV)
+    data = normal(3, steps, 3, heads + 2 * kv, dim, dtype=BF16).to(DEV)
+
+    def step(x, cache, batch, positions):
+        q = attention.append(x[:, heads:heads + kv], x[:, heads + kv:], cache, batch, q=x[:, :heads], positions=positions,
+                             turns=table, q_weight=w, k_weight=w)
+        return attention.attend(q, cache, batch)
+
+    def state():
+        cache = attention.Cache(*(t.clone() for t in first))
+        return cache, whole._replace(lengths=i32(*lengths).to(DEV)), i32(*(n - 1 for n in lengths)).to(DEV)
+    cache, batch, positions = state()
+    eager = []
+    for i in range(steps):
+        eager.append(step(data[i], cache, batch, positions).clone())
+        batch.lengths.add_(1), positions.add_(1)
+    kept = [t.clone() for t in cache]
+    cache, batch, positions = state()
+    x = data[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, cache, batch, positions)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, cache, batch, positions)
+    for a, b in zip(cache, first):
+        a.view(torch.int8).copy_(b.view(torch.int8))
+    for i in range(steps):
+        x.copy_(data[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[i])
+        batch.lengths.add_(1), positions.add_(1)
+    assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(kept, cache))
+
+
+def test_declined():
+    cache = attention.new_cache(2, 1, 96, device=DEV)
+    batch, _ = make_batch([3], [1], blocks=2)
+    x = torch.zeros(1, 1, 96, dtype=F16, device=DEV)
+    assert attention.attend(x, cache, batch) is None and attention.append(x, x, cache, batch) is None
+    assert attention.read(cache, batch) is None and attention.norm_rope(x, x) is None
+    cache = attention.new_cache(2, 1, 64, device=DEV)
+    assert attention.attend(torch.zeros(1, 1, 64, device=DEV), cache, batch) is None

@@ -348,7 +348,8 @@ def run(state):
             q = attention.append(state["k"], state["v"], cache, batch, q=state["q"], positions=state["positions"],
                                  turns=state["turns"], q_weight=state["q_weight"], k_weight=state["k_weight"], eps=EPS)
         else:
-            q = attention.append(state["k"], state["v"], cache, batch)
+            q = None
+            attention.append(state["k"], state["v"], cache, batch)
         k, v = attention.read(cache, batch, tail=state["tail"], dtype=DTYPE[case["dtype"]])
         return {"q": q, "k": k, "v": v, "k_scale": cache.k_scale, "v_scale": cache.v_scale}
     if kind == "rotate":

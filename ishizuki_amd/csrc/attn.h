@@ -179,6 +179,51 @@ DEV void unit_norm(float *x, const float *w, int ca, int cb, float eps) {
   for (int i = 0; i < 16; i++) x[i] *= r * w[i < 8 ? ca + i : cb + i - 8];
 }
 
+// ---------------------------------------------------------------- attention
+struct Call {
+  const void *q;
+  int64_t row, head;  // strides in values
+  void *out;          // [rows][heads][dim]
+  int heads, group;   // q heads, and of them to a head of the cache
+  float scale;        // of the logits, times log2 e
+  int causal, window;
+  int splits;
+  float *part;  // [splits][rows][heads][dim]: sums in units of their own maximum
+  float2 *ml;   // [splits][rows][heads]: that maximum (of log2 weights) and the sum of weights
+};
+
+// q's sixteen values of a lane, as matrix operands: dims 64 e + 16 quad .. + 15 for each e of D / 64, bf16 as fp16 with a
+// power of two for the row (see act_prepare), which the returned factor of its logits holds.
+template <int D, int DT>
+DEV float load_query(const Call &c, int64_t row, int head, int quad, h8 *q) {
+  constexpr int C = D / 64;
+  const size_t at = (size_t)(row * c.row + head * c.head) + 16 * quad;
+  u4 v[2 * C];
+#pragma unroll
+  for (int e = 0; e < 2 * C; e++) v[e] = *(const u4 *)((const uint16_t *)c.q + at + 64 * (e / 2) + 8 * (e % 2));
+  float scale = c.scale;
+  if (DT == ISHZ_DT_BF16) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 2 * C; e++) m = bf16_absmax(v[e], m);
+    const auto a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    m = max((uint32_t)a[0], (uint32_t)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    const int x = bf16_row_exponent(max((uint32_t)b[0], (uint32_t)b[1]));
+    const float down = ldexpf(1.0f, -x);
+#pragma unroll
+    for (int e = 0; e < 2 * C; e++) v[e] = bf16_to_half8(v[e], down);
+    scale *= ldexpf(1.0f, x);
+  }
+#pragma unroll
+  for (int e = 0; e < 2 * C; e++) q[e] = as_h8(v[e]);
+  return scale;
+}
+
+// tile_kernel (attn_tile.hip): packed rows of a workgroup, and its launch over `tiles` of them a sequence.
+int tile_rows(int dim);
+void launch_tile(const Call &c, const Pool &pool, const Rows &rows, int format, int dtype, int tiles, uint32_t total, hipStream_t st);
+
 // What every call on the cache refuses (attn_cache.hip).
 int check_pool(const void *k, const void *v, const float *ks, const float *vs, int format, int blocks, int heads, int dim);
 int check_rows(const int32_t *table, const int32_t *lengths, const int32_t *starts, int sequences, int width, int rows);

@@ -4,18 +4,6 @@
 #include "attn.h"
 
 namespace attn {
-struct Call {
-  const void *q;
-  int64_t row, head;  // strides in values
-  void *out;          // [rows][heads][dim]
-  int heads, group;   // q heads, and of them to a head of the cache
-  float scale;        // of the logits, times log2 e
-  int causal, window;
-  int splits;
-  float *part;  // [splits][rows][heads][dim]: sums in units of their own maximum
-  float2 *ml;   // [splits][rows][heads]: that maximum (of log2 weights) and the sum of weights
-};
-
 // ---------------------------------------------------------------- few rows: the cache streams past them
 // The rows of a sequence and its q heads of one cache head are packed, 16 to a tile. A wave takes 64 tokens (one
 // block) at a time, from memory straight into matrix operands:
@@ -49,26 +37,7 @@ __global__ __launch_bounds__(256) void stream_kernel(Call c, Pool pool, Rows row
     const int r = min(r0 + 16 * t + col, packed - 1), i = r / c.group;
     end[t] = c.causal ? base + i + 1 : length;
     begin[t] = c.window ? max(base + i + 1 - c.window, 0) : 0;
-    const size_t at = (size_t)((int64_t)(row0 + i) * c.row + (int64_t)(kvh * c.group + r % c.group) * c.head) + 16 * quad;
-    u4 v[2 * C];
-#pragma unroll
-    for (int e = 0; e < 2 * C; e++) v[e] = *(const u4 *)((const uint16_t *)c.q + at + 64 * (e / 2) + 8 * (e % 2));
-    scale[t] = c.scale;
-    if (DT == ISHZ_DT_BF16) {  // as fp16 with a power of two for each row (see act_prepare)
-      uint32_t m = 0;
-#pragma unroll
-      for (int e = 0; e < 2 * C; e++) m = bf16_absmax(v[e], m);
-      const auto a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
-      m = max((uint32_t)a[0], (uint32_t)a[1]);
-      const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
-      const int x = bf16_row_exponent(max((uint32_t)b[0], (uint32_t)b[1]));
-      const float down = ldexpf(1.0f, -x);
-#pragma unroll
-      for (int e = 0; e < 2 * C; e++) v[e] = bf16_to_half8(v[e], down);
-      scale[t] *= ldexpf(1.0f, x);
-    }
-#pragma unroll
-    for (int e = 0; e < 2 * C; e++) q[t][e] = as_h8(v[e]);
+    scale[t] = load_query<D, DT>(c, row0 + i, kvh * c.group + r % c.group, quad, q[t]);
   }
 
   // blocks that some row sees; those that every row sees whole need no mask
@@ -248,16 +217,19 @@ __global__ __launch_bounds__(256) void join_kernel(Call c, const int32_t *starts
 
 // How a call is divided: packed rows to a workgroup, and splits of the cache.
 struct Plan {
-  int row_tiles, tiles, splits;
+  int row_tiles, tiles, splits;  // row_tiles 0: tile_kernel
 };
 static Plan plan(int q_heads, int heads, int dim, int sequences, int max_rows, int max_length) {
   Plan p;
   const int64_t packed = (int64_t)max_rows * (q_heads / heads);
-  p.row_tiles = packed <= 16 ? 1 : packed <= 32 || dim == 256 ? 2 : 4;
-  p.tiles = (int)((packed + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
+  p.row_tiles = packed <= 16 ? 1 : packed <= 32 ? 2 : 0;
+  const int per = p.row_tiles ? 16 * p.row_tiles : tile_rows(dim);
+  p.tiles = (int)((packed + per - 1) / per);
   const int64_t groups = (int64_t)sequences * heads * p.tiles;
   const int64_t blocks = ((int64_t)max_length + BLOCK - 1) / BLOCK;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + groups - 1) / std::max<int64_t>(groups, 1), (blocks + 3) / 4, 64}));
+  const int64_t want = p.row_tiles ? 1024 : 512;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want + groups - 1) / std::max<int64_t>(groups, 1), (blocks + 3) / 4, 64}));
+  if (!p.row_tiles && groups * 2 > want) p.splits = 1;
   return p;
 }
 }  // namespace attn
@@ -302,13 +274,13 @@ extern "C" int ishz_kv_attend(const void *q, int64_t q_row, int64_t q_head, int 
 #define ISHZ_STREAM(D, F, T, RT)                                                                                         \
   hipLaunchKernelGGL(HIP_KERNEL_NAME(stream_kernel<D, F, T, RT>), dim3((uint32_t)total), dim3(256), 0, ishz::S(stream), c, pool, r, \
                      p.tiles)
-#define ISHZ_STREAM_RT(D, F, T) \
-  if (p.row_tiles == 1) ISHZ_STREAM(D, F, T, 1); else if (p.row_tiles == 2) ISHZ_STREAM(D, F, T, 2); else ISHZ_STREAM(D, F, T, 4)
-#define ISHZ_STREAM_D(F, T)                                                 \
-  if (dim == 64) { ISHZ_STREAM_RT(64, F, T); }                              \
-  else if (dim == 128) { ISHZ_STREAM_RT(128, F, T); }                       \
-  else if (p.row_tiles == 1) ISHZ_STREAM(256, F, T, 1); else ISHZ_STREAM(256, F, T, 2)
-  if (format == ISHZ_KV_INT8) {
+#define ISHZ_STREAM_RT(D, F, T) if (p.row_tiles == 1) ISHZ_STREAM(D, F, T, 1); else ISHZ_STREAM(D, F, T, 2)
+#define ISHZ_STREAM_D(F, T)                          \
+  if (dim == 64) { ISHZ_STREAM_RT(64, F, T); }       \
+  else if (dim == 128) { ISHZ_STREAM_RT(128, F, T); } \
+  else { ISHZ_STREAM_RT(256, F, T); }
+  if (!p.row_tiles) launch_tile(c, pool, r, format, dtype, p.tiles, (uint32_t)total, ishz::S(stream));
+  else if (format == ISHZ_KV_INT8) {
     if (dtype == ISHZ_DT_F16) { ISHZ_STREAM_D(ISHZ_KV_INT8, ISHZ_DT_F16); } else { ISHZ_STREAM_D(ISHZ_KV_INT8, ISHZ_DT_BF16); }
   } else {
     if (dtype == ISHZ_DT_F16) { ISHZ_STREAM_D(ISHZ_KV_E4M3, ISHZ_DT_F16); } else { ISHZ_STREAM_D(ISHZ_KV_E4M3, ISHZ_DT_BF16); }

@@ -1,0 +1,259 @@
+// Attention over the 8-bit cache for many rows: prompts, drafted tokens of wide groups, cross attention.
+#include "attn.h"
+
+namespace attn {
+// W waves of 16 RT packed rows (a sequence's rows and its q heads of one cache head) pass the cache's blocks together.
+// Each block is decoded to fp16 once for all of them, into LDS in the order in which the matrix operands are read (a
+// wave's 64 lanes read 1 KB in a row), two blocks deep: while one is worked on, the next one's codes are on their way
+// in registers. As in stream_kernel S^T = K Q^T leaves a lane the weights of 16 consecutive tokens of a row, which are
+// the operands of O^T += V^T P^T as they are.
+//
+// Sums stay in the units of a reference that is only moved when a logit passes it by 2^8 (weights stay below fp16's
+// largest), and of a value scale `unit` that blocks' scales are 1..16 of: log2 of that ratio is added to the block's
+// logits, so that nothing but the matrix units touches the sums. A block outside 1..16 moves the unit, which stays above
+// 2^-80 of the largest scale (the sums' 2^41 then stay finite).
+template <int D, int FMT, int DT, int RT, int W>
+__global__ __launch_bounds__(64 * W, RT * D > 384 ? 1 : 2) void tile_kernel(Call c, Pool pool, Rows rows, int tiles) {
+  constexpr int C = D / 64, V = D / 16;
+  extern __shared__ h8 held[];  // [2][16 C operands][64]
+  int id = blockIdx.x;
+  const int kvh = id % pool.heads;
+  id /= pool.heads;
+  const int split = id % c.splits;
+  id /= c.splits;
+  // the last rows of a causal call see most and start first
+  const int tile = tiles - 1 - id / rows.sequences, seq = id % rows.sequences;
+  const int row0 = rows.first(seq), n = rows.count(seq), length = rows.length(seq), base = length - n;
+  const int packed = n * c.group, r0 = tile * (16 * RT * W);
+  if (r0 >= packed) return;
+  const int wave = wave_id(), lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  const int w0 = r0 + wave * (16 * RT);
+
+  h8 q[RT][2 * C];
+  float scale[RT];
+  int end[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const int r = min(w0 + 16 * t + col, packed - 1), i = r / c.group;
+    end[t] = c.causal ? base + i + 1 : length;
+    scale[t] = load_query<D, DT>(c, row0 + i, kvh * c.group + r % c.group, quad, q[t]);
+  }
+  const int window = c.window ? c.window : INT32_MAX;  // a row sees tokens end - window .. end - 1
+
+  // blocks that some row of the workgroup sees, and the tokens that some, or all, of the wave's rows do
+  const int i0 = r0 / c.group, i1 = (min(r0 + 16 * RT * W, packed) - 1) / c.group;
+  const int last = c.causal ? base + i1 + 1 : length, from = c.window ? max(base + i0 + 1 - c.window, 0) : 0;
+  const int b0 = from / BLOCK, b1 = max((last + BLOCK - 1) / BLOCK, b0);
+  const int each = (b1 - b0 + c.splits - 1) / c.splits;
+  const int first = b0 + split * each, stop = min(first + each, b1);
+  const int j0 = w0 / c.group, j1 = (min(w0 + 16 * RT, packed) - 1) / c.group;
+  const int some0 = c.window ? max(base + j0 + 1 - c.window, 0) : 0;
+  const int some1 = w0 >= packed ? 0 : c.causal ? base + j1 + 1 : length;
+  const int whole0 = c.window ? max(base + j1 + 1 - c.window, 0) : 0, whole1 = c.causal ? base + j0 + 1 : length;
+
+  // The operands of a block, 1 KB each: K's (t, dims 32 x ..) for x < 2 C, then V's (d, tokens 8 x of each quad's 16 ..).
+  // A wave decodes 2 C of K's (of tile t = wave % 4) and 2 C of V's, or with eight waves one or the other.
+  constexpr bool BOTH = W == 4;
+  u4 raw[BOTH ? 2 * C : C];
+  const int part = wave & 3, is_v = BOTH ? 0 : wave >> 2;
+  const uint32_t k_at = (16 * (col >> 2) + 4 * part + (col & 3)) * D + 16 * quad, v_at = (16 * C * part + col) * BLOCK + 16 * quad;
+  const auto fetch = [&](int block) {
+    const uint8_t *const kt = pool.k + pool.tile(block, kvh), *const vt = pool.v + pool.tile(block, kvh);
+    if (BOTH || !is_v) {
+#pragma unroll
+      for (int i = 0; i < C; i++) raw[i] = *(const u4 *)(kt + k_at + 64 * i);
+    }
+    if (BOTH || is_v) {
+#pragma unroll
+      for (int i = 0; i < C; i++) raw[BOTH ? C + i : i] = *(const u4 *)(vt + v_at + 16 * BLOCK * i);
+    }
+  };
+  const auto put = [&](int b, int buffer) {
+    h8 *const to = held + buffer * (16 * C * 64) + part * (2 * C * 64) + (BOTH ? 0 : is_v * (8 * C * 64)) + lane;
+    // past the sequence's end a block holds whatever was there: an e4m3 NaN times a weight of 0 must not count
+    if (FMT == ISHZ_KV_E4M3 && (BOTH || is_v) && b * BLOCK + BLOCK > length) {
+#pragma unroll
+      for (int i = 0; i < C; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int left = length - (b * BLOCK + 16 * quad + 4 * e);
+          raw[BOTH ? C + i : i][e] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << 8 * left) - 1;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < (BOTH ? 2 * C : C); i++) {
+      h8 *const x = to + (i < C ? i * 128 : 8 * C * 64 + (i - C) * 128);
+      x[0] = decode8<FMT>(raw[i].x, raw[i].y);
+      x[64] = decode8<FMT>(raw[i].z, raw[i].w);
+    }
+  };
+
+  f4 o[RT][V];
+  float m[RT], l[RT], unit = 0x1p-100f, largest = 0;
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    m[t] = -3e38f, l[t] = 0;
+#pragma unroll
+    for (int d = 0; d < V; d++) o[t][d] = f4{0, 0, 0, 0};
+  }
+  int block = first < stop ? rows.block(seq, first, pool.blocks) : -1;
+  if (block >= 0) {
+    fetch(block);
+    put(first, 0);
+  }
+  __syncthreads();
+  for (int b = first; b < stop; b++) {
+    const int next = b + 1 < stop ? rows.block(seq, b + 1, pool.blocks) : -1;
+    if (next >= 0) fetch(next);
+    const int p0 = b * BLOCK;
+    if (block >= 0 && p0 < some1 && p0 + BLOCK > some0) {
+      const float vs = pool.vs[pool.scale(block, kvh)], none = vs - vs;
+      // a value scale of no number makes the logits none, of the rows that see the block
+      const float ks = pool.ks[pool.scale(block, kvh)] + none, vb = none == 0 ? vs : unit;
+      const h8 *const at = held + ((b - first) & 1) * (16 * C * 64) + lane;
+      h8 a = at[0], a2 = at[64];
+      f4 s[RT][4];
+#pragma unroll
+      for (int x = 0; x < 4 * C; x++) {
+        const h8 y = at[(2 * x + 2) * 64], y2 = at[(2 * x + 3) * 64];
+        __builtin_amdgcn_sched_barrier(0);
+        const int t = x / C;
+#pragma unroll
+        for (int r = 0; r < RT; r++) s[r][t] = mfma32(a, q[r][2 * (x % C)], x % C ? s[r][t] : f4{0, 0, 0, 0});
+#pragma unroll
+        for (int r = 0; r < RT; r++) s[r][t] = mfma32(a2, q[r][2 * (x % C) + 1], s[r][t]);
+        a = y, a2 = y2;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      float f[RT];
+#pragma unroll
+      for (int r = 0; r < RT; r++) f[r] = scale[r] * ks;
+      if (p0 < whole0 || p0 + BLOCK > whole1) {
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          const int before = end[r] - 1 - (p0 + 16 * quad);  // tokens between the lane's first and the row's last
+#pragma unroll
+          for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              s[r][t][i] = before >= 4 * t + i && before - (4 * t + i) < window ? s[r][t][i] * f[r] : -__builtin_inff();
+          f[r] = 1;
+        }
+      }
+      float top[RT];
+      bool move = false;
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        float x = s[r][0][0];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) x = fmaxf(x, s[r][t][i]);
+        top[r] = x * f[r];
+        move |= top[r] > m[r] + 8.0f;
+      }
+      const float was = unit;
+      largest = fmaxf(largest, vb);
+      if (vb < unit || vb > 16.0f * unit) unit = fmaxf(fmaxf(0.25f * vb, 0x1p-80f * largest), 0x1p-100f);
+      if (unit != was || __any(move)) {
+        const float units = was / unit;
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          float x = fmaxf(top[r], m[r]);
+          x = fmaxf(x, lane_xor16(x));
+          x = fmaxf(x, lane_xor32(x));
+          const float alpha = __builtin_amdgcn_exp2f(m[r] - x);
+          m[r] = x;
+          l[r] *= alpha;
+#pragma unroll
+          for (int d = 0; d < V; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[r][d][i] *= alpha * units;
+        }
+      }
+      const float ratio = vb / unit, shift = __builtin_amdgcn_logf(ratio), back = 1.0f / ratio;
+      h8 p[RT][2];
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        const float ref = shift - m[r];
+        float sum = 0;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          typedef float f2 __attribute__((ext_vector_type(2)));
+          const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][0], f[r], ref));
+          const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][1], f[r], ref));
+          const float w2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][2], f[r], ref));
+          const float w3 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][3], f[r], ref));
+          sum += (w0 + w1) + (w2 + w3);
+          // Weights are rounded to fp16 for the matrix units: 2^-12 of each, the sums stay in 32 bits.
+          const h2 lo = __builtin_convertvector((f2{w0, w1}), h2), hi = __builtin_convertvector((f2{w2, w3}), h2);
+          p[r][t / 2][4 * (t % 2)] = lo.x, p[r][t / 2][4 * (t % 2) + 1] = lo.y;
+          p[r][t / 2][4 * (t % 2) + 2] = hi.x, p[r][t / 2][4 * (t % 2) + 3] = hi.y;
+        }
+        l[r] += sum * back;
+      }
+#pragma unroll
+      for (int d = 0; d < V; d++) {
+        h8 y = a, y2 = a2;
+        if (d + 1 < V) y = at[(8 * C + 2 * d + 2) * 64], y2 = at[(8 * C + 2 * d + 3) * 64];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < RT; r++) o[r][d] = mfma32(a, p[r][0], o[r][d]);
+#pragma unroll
+        for (int r = 0; r < RT; r++) o[r][d] = mfma32(a2, p[r][1], o[r][d]);
+        a = y, a2 = y2;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (next >= 0) put(b + 1, (b + 1 - first) & 1);
+    block = next;
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    float sum = l[t];
+    sum += lane_xor16(sum);
+    sum += lane_xor32(sum);
+    const int r = w0 + 16 * t + col;
+    if (r >= packed) continue;
+    const size_t at = (size_t)(row0 + r / c.group) * c.heads + kvh * c.group + r % c.group;
+    const float by = c.splits > 1 ? unit : sum == 0 ? 0.0f : unit / sum;
+    const size_t to = (size_t)split * rows.rows * c.heads + at;
+#pragma unroll
+    for (int d = 0; d < V; d++) {
+      f4 x = o[t][d];
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] *= by;
+      if (c.splits == 1) *(u2 *)((uint16_t *)c.out + at * D + 16 * d + 4 * quad) = u2{narrow2<DT>(x[0], x[1]), narrow2<DT>(x[2], x[3])};
+      else *(f4 *)(c.part + to * D + 16 * d + 4 * quad) = x;
+    }
+    if (c.splits > 1 && quad == 0) c.ml[to] = float2{m[t], sum};
+  }
+}
+
+// Row tiles of a wave: the most whose sums, queries and logits (24, 40 or 88 registers each) leave two waves a SIMD (for
+// heads of 256: one), for each operand read from LDS feeds that many products.
+constexpr int TILE_WAVES = 4;
+template <int D>
+constexpr int ROW_TILES = D == 64 ? 4 : D == 128 ? 3 : 2;
+int tile_rows(int dim) { return 16 * TILE_WAVES * (dim == 64 ? ROW_TILES<64> : dim == 128 ? ROW_TILES<128> : ROW_TILES<256>); }
+
+template <int D, int FMT, int DT>
+static void launch(const Call &c, const Pool &pool, const Rows &rows, int tiles, uint32_t total, hipStream_t st) {
+  constexpr int RT = ROW_TILES<D>, W = TILE_WAVES;
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_kernel<D, FMT, DT, RT, W>), dim3(total), dim3(64 * W), 2 * 16 * (D / 64) * 1024, st, c,
+                     pool, rows, tiles);
+}
+void launch_tile(const Call &c, const Pool &pool, const Rows &rows, int format, int dtype, int tiles, uint32_t total, hipStream_t st) {
+#define ISHZ_TILE_D(F, T)                                               \
+  if (pool.dim == 64) launch<64, F, T>(c, pool, rows, tiles, total, st);     \
+  else if (pool.dim == 128) launch<128, F, T>(c, pool, rows, tiles, total, st); \
+  else launch<256, F, T>(c, pool, rows, tiles, total, st)
+  if (format == ISHZ_KV_INT8) {
+    if (dtype == ISHZ_DT_F16) { ISHZ_TILE_D(ISHZ_KV_INT8, ISHZ_DT_F16); } else { ISHZ_TILE_D(ISHZ_KV_INT8, ISHZ_DT_BF16); }
+  } else {
+    if (dtype == ISHZ_DT_F16) { ISHZ_TILE_D(ISHZ_KV_E4M3, ISHZ_DT_F16); } else { ISHZ_TILE_D(ISHZ_KV_E4M3, ISHZ_DT_BF16); }
+  }
+}
+}  // namespace attn

@@ -107,7 +107,7 @@ def test_turns():
             exact = math.fmod(position * 1e6 ** (-2.0 * i / 64) / (2 * math.pi), 1.0)
             got = (position * bits % (1 << 64)) / 2.0 ** 64
             off = abs(got - exact) % 1.0
-            assert min(off, 1 - off) < 2.0 ** -20 if position == 2 ** 31 - 1 else 2.0 ** -30
+            assert min(off, 1 - off) < (2.0 ** -20 if position == 2 ** 31 - 1 else 2.0 ** -30)
     assert torch.equal(attention.turns(inv_freq=[1.0, 0.5], device="cpu"), attention.turns(inv_freq=torch.tensor([1.0, 0.5]), device="cpu"))
 
 

@@ -192,7 +192,7 @@ struct Call {
   float2 *ml;   // [splits][rows][heads]: that maximum (of log2 weights) and the sum of weights
 };
 
-// q's sixteen values of a lane, as matrix operands: dims 64 e + 16 quad .. + 15 for each e of D / 64, bf16 as fp16 with a
+// A lane's values of a row of q, as matrix operands: dims 64 e + 16 quad .. + 15 for each e of D / 64; bf16 as fp16 with a
 // power of two for the row (see act_prepare), which the returned factor of its logits holds.
 template <int D, int DT>
 DEV float load_query(const Call &c, int64_t row, int head, int quad, h8 *q) {

@@ -2,18 +2,23 @@
 #include "attn.h"
 
 namespace attn {
-// W waves of 16 RT packed rows (a sequence's rows and its q heads of one cache head) pass the cache's blocks together.
+// Eight waves of 16 RT packed rows (a sequence's rows and its q heads of one cache head) pass the cache's blocks together.
 // Each block is decoded to fp16 once for all of them, into LDS in the order in which the matrix operands are read (a
-// wave's 64 lanes read 1 KB in a row), two blocks deep: while one is worked on, the next one's codes are on their way
-// in registers. As in stream_kernel S^T = K Q^T leaves a lane the weights of 16 consecutive tokens of a row, which are
-// the operands of O^T += V^T P^T as they are.
+// wave's 64 lanes read 1 KB in a row: 255 bytes a clock measured, rows of 272 bytes 128), two blocks deep: while one is
+// worked on, the next one's codes are on their way in registers. As in stream_kernel S^T = K Q^T leaves a lane the
+// weights of 16 consecutive tokens of a row, which are the operands of O^T += V^T P^T as they are.
 //
 // Sums stay in the units of a reference that is only moved when a logit passes it by 2^8 (weights stay below fp16's
-// largest), and of a value scale `unit` that blocks' scales are 1..16 of: log2 of that ratio is added to the block's
-// logits, so that nothing but the matrix units touches the sums. A block outside 1..16 moves the unit, which stays above
-// 2^-80 of the largest scale (the sums' 2^41 then stay finite).
-template <int D, int FMT, int DT, int RT, int W>
-__global__ __launch_bounds__(64 * W, RT * D > 384 ? 1 : 2) void tile_kernel(Call c, Pool pool, Rows rows, int tiles) {
+// largest), and of a value scale `unit` that blocks' scales are 1..255 of: log2 of that ratio is added to the block's
+// logits, so that nothing but the matrix units touches the sums. A block outside 1..255 moves the unit, which stays above
+// 2^-80 of the largest scale (the sums' 2^45 then stay finite).
+//
+// Power bounds it: these products alone, from registers, run at 1970 TFLOP/s on such values (1700 as 32x32x16) where the
+// clock would allow 2500, and a library product of 8192 x 8192 x 8192 at 1250 to 1500; 8192 tokens of 32 heads over 8 of
+// 128, causal, take 535 us (1030 TFLOP/s). That time is within 4 % for 16 to 48 rows a wave, products of either
+// shape, vector operations dealt between the products or not, and codes unpacked by a pass before.
+template <int D, int FMT, int DT, int RT>
+__global__ __launch_bounds__(512, 2) void tile_kernel(Call c, Pool pool, Rows rows, int tiles) {
   constexpr int C = D / 64, V = D / 16;
   extern __shared__ h8 held[];  // [2][16 C operands][64]
   int id = blockIdx.x;
@@ -24,7 +29,7 @@ __global__ __launch_bounds__(64 * W, RT * D > 384 ? 1 : 2) void tile_kernel(Call
   // the last rows of a causal call see most and start first
   const int tile = tiles - 1 - id / rows.sequences, seq = id % rows.sequences;
   const int row0 = rows.first(seq), n = rows.count(seq), length = rows.length(seq), base = length - n;
-  const int packed = n * c.group, r0 = tile * (16 * RT * W);
+  const int packed = n * c.group, r0 = tile * 128 * RT;
   if (r0 >= packed) return;
   const int wave = wave_id(), lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
   const int w0 = r0 + wave * (16 * RT);
@@ -41,7 +46,7 @@ __global__ __launch_bounds__(64 * W, RT * D > 384 ? 1 : 2) void tile_kernel(Call
   const int window = c.window ? c.window : INT32_MAX;  // a row sees tokens end - window .. end - 1
 
   // blocks that some row of the workgroup sees, and the tokens that some, or all, of the wave's rows do
-  const int i0 = r0 / c.group, i1 = (min(r0 + 16 * RT * W, packed) - 1) / c.group;
+  const int i0 = r0 / c.group, i1 = (min(r0 + 128 * RT, packed) - 1) / c.group;
   const int last = c.causal ? base + i1 + 1 : length, from = c.window ? max(base + i0 + 1 - c.window, 0) : 0;
   const int b0 = from / BLOCK, b1 = max((last + BLOCK - 1) / BLOCK, b0);
   const int each = (b1 - b0 + c.splits - 1) / c.splits;
@@ -51,65 +56,90 @@ __global__ __launch_bounds__(64 * W, RT * D > 384 ? 1 : 2) void tile_kernel(Call
   const int some1 = w0 >= packed ? 0 : c.causal ? base + j1 + 1 : length;
   const int whole0 = c.window ? max(base + j1 + 1 - c.window, 0) : 0, whole1 = c.causal ? base + j0 + 1 : length;
 
-  // The operands of a block, 1 KB each: K's (t, dims 32 x ..) for x < 2 C, then V's (d, tokens 8 x of each quad's 16 ..).
-  // A wave decodes 2 C of K's (of tile t = wave % 4) and 2 C of V's, or with eight waves one or the other.
-  constexpr bool BOTH = W == 4;
-  u4 raw[BOTH ? 2 * C : C];
-  const int part = wave & 3, is_v = BOTH ? 0 : wave >> 2;
-  const uint32_t k_at = (16 * (col >> 2) + 4 * part + (col & 3)) * D + 16 * quad, v_at = (16 * C * part + col) * BLOCK + 16 * quad;
+  // The operands of a block, 1 KB each: 8 C of K (tile t of the tokens, dims), then 8 C of V (dims, tokens). Waves 0..3
+  // decode K's, 4..7 V's.
+  u4 raw[C];
+  const int part = wave & 3;
+  const bool is_v = wave >> 2;
+  const uint32_t from_at = is_v ? (16 * C * part + col) * BLOCK + 16 * quad : (16 * (col >> 2) + 4 * part + (col & 3)) * D + 16 * quad;
   const auto fetch = [&](int block) {
-    const uint8_t *const kt = pool.k + pool.tile(block, kvh), *const vt = pool.v + pool.tile(block, kvh);
-    if (BOTH || !is_v) {
+    const uint8_t *const x = (is_v ? pool.v : pool.k) + pool.tile(block, kvh) + from_at;
 #pragma unroll
-      for (int i = 0; i < C; i++) raw[i] = *(const u4 *)(kt + k_at + 64 * i);
-    }
-    if (BOTH || is_v) {
-#pragma unroll
-      for (int i = 0; i < C; i++) raw[BOTH ? C + i : i] = *(const u4 *)(vt + v_at + 16 * BLOCK * i);
-    }
+    for (int i = 0; i < C; i++) raw[i] = *(const u4 *)(x + (is_v ? 16 * BLOCK : 64) * i);
   };
-  const auto put = [&](int b, int buffer) {
-    h8 *const to = held + buffer * (16 * C * 64) + part * (2 * C * 64) + (BOTH ? 0 : is_v * (8 * C * 64)) + lane;
+  const auto put = [&](int b) {
+    h8 *const to = held + ((b - first) & 1) * (16 * C * 64) + wave * (2 * C * 64) + lane;
     // past the sequence's end a block holds whatever was there: an e4m3 NaN times a weight of 0 must not count
-    if (FMT == ISHZ_KV_E4M3 && (BOTH || is_v) && b * BLOCK + BLOCK > length) {
+    if (FMT == ISHZ_KV_E4M3 && is_v && b * BLOCK + BLOCK > length) {
 #pragma unroll
       for (int i = 0; i < C; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int left = length - (b * BLOCK + 16 * quad + 4 * e);
-          raw[BOTH ? C + i : i][e] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << 8 * left) - 1;
+          raw[i][e] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << 8 * left) - 1;
         }
     }
 #pragma unroll
-    for (int i = 0; i < (BOTH ? 2 * C : C); i++) {
-      h8 *const x = to + (i < C ? i * 128 : 8 * C * 64 + (i - C) * 128);
-      x[0] = decode8<FMT>(raw[i].x, raw[i].y);
-      x[64] = decode8<FMT>(raw[i].z, raw[i].w);
+    for (int i = 0; i < C; i++) {
+      to[i * 128] = decode8<FMT>(raw[i].x, raw[i].y);
+      to[i * 128 + 64] = decode8<FMT>(raw[i].z, raw[i].w);
     }
   };
 
   f4 o[RT][V];
-  float m[RT], l[RT], unit = 0x1p-100f, largest = 0;
+  float m[RT], l[RT];
+  float unit = 0x1p-100f, largest = 0;
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     m[t] = -3e38f, l[t] = 0;
 #pragma unroll
     for (int d = 0; d < V; d++) o[t][d] = f4{0, 0, 0, 0};
   }
-  int block = first < stop ? rows.block(seq, first, pool.blocks) : -1;
+  // The numbers of 64 blocks from `from_b` on and what their scales come to, a lane each: read one by one where they are
+  // needed, they would be two dependent loads' latency in every step. The unit stays as it is up to `until`.
+  int ids = -1, from_b = first, until = first;
+  float kss = 0, vss = 0, logs = 0, backs = 1;
+  const auto refill = [&](int b) {
+    from_b = b;
+    ids = b + lane < stop ? rows.block(seq, b + lane, pool.blocks) : -1;
+    const size_t x = pool.scale(max(ids, 0), kvh);
+    const float v = pool.vs[x], none = v - v;
+    // a value scale of no number makes the logits none, of the rows that see the block
+    kss = ids < 0 ? 0.0f : pool.ks[x] + none;
+    vss = ids < 0 || none != 0 ? -1.0f : fmaxf(v, 0x1p-126f);
+    until = b;
+  };
+  const auto lane_value = [&](float v, int b) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), b - from_b));
+  };
+  const auto block_at = [&](int b) { return __builtin_amdgcn_readlane(ids, b - from_b); };
+  // The unit of blocks b .. until - 1.
+  const auto set_unit = [&](int b) {
+    const float v = lane_value(vss, b);
+    if (v > 0) largest = fmaxf(largest, v), unit = fmaxf(fmaxf(v * 0x1p-4f, 0x1p-80f * largest), 0x1p-100f);
+    const float ratio = vss < 0 ? 1.0f : fmaxf(vss / unit, 0x1p-64f);
+    logs = __builtin_amdgcn_logf(ratio), backs = 1.0f / ratio;
+    const bool out = ratio > 255.0f || (ratio < 1.0f && vss > 0x1p-76f * largest && vss > 0x1p-100f);
+    const uint64_t off = __ballot(out) >> (b - from_b) >> 1;
+    until = off ? b + 1 + __builtin_ctzll(off) : from_b + 64;
+  };
+
+  refill(first);
+  int block = first < stop ? block_at(first) : -1;
   if (block >= 0) {
     fetch(block);
-    put(first, 0);
+    put(first);
   }
   __syncthreads();
   for (int b = first; b < stop; b++) {
-    const int next = b + 1 < stop ? rows.block(seq, b + 1, pool.blocks) : -1;
+    if (b - from_b > 62) refill(b);
+    const int next = block_at(b + 1);
     if (next >= 0) fetch(next);
     const int p0 = b * BLOCK;
     if (block >= 0 && p0 < some1 && p0 + BLOCK > some0) {
-      const float vs = pool.vs[pool.scale(block, kvh)], none = vs - vs;
-      // a value scale of no number makes the logits none, of the rows that see the block
-      const float ks = pool.ks[pool.scale(block, kvh)] + none, vb = none == 0 ? vs : unit;
+      const float was = unit;
+      if (b >= until) set_unit(b);
+      const float ks = lane_value(kss, b), shift = lane_value(logs, b), back = lane_value(backs, b);
       const h8 *const at = held + ((b - first) & 1) * (16 * C * 64) + lane;
       h8 a = at[0], a2 = at[64];
       f4 s[RT][4];
@@ -152,9 +182,6 @@ __global__ __launch_bounds__(64 * W, RT * D > 384 ? 1 : 2) void tile_kernel(Call
         top[r] = x * f[r];
         move |= top[r] > m[r] + 8.0f;
       }
-      const float was = unit;
-      largest = fmaxf(largest, vb);
-      if (vb < unit || vb > 16.0f * unit) unit = fmaxf(fmaxf(0.25f * vb, 0x1p-80f * largest), 0x1p-100f);
       if (unit != was || __any(move)) {
         const float units = was / unit;
 #pragma unroll
@@ -166,12 +193,14 @@ __global__ __launch_bounds__(64 * W, RT * D > 384 ? 1 : 2) void tile_kernel(Call
           m[r] = x;
           l[r] *= alpha;
 #pragma unroll
-          for (int d = 0; d < V; d++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[r][d][i] *= alpha * units;
+          for (int d = 0; d < V; d++) {  // one after another: the compiler holds all of them twice otherwise
+            f4 y = o[r][d] * (alpha * units);
+            asm volatile("" : "+v"(y));
+            o[r][d] = y;
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
       }
-      const float ratio = vb / unit, shift = __builtin_amdgcn_logf(ratio), back = 1.0f / ratio;
       h8 p[RT][2];
 #pragma unroll
       for (int r = 0; r < RT; r++) {
@@ -205,7 +234,7 @@ __global__ __launch_bounds__(64 * W, RT * D > 384 ? 1 : 2) void tile_kernel(Call
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (next >= 0) put(b + 1, (b + 1 - first) & 1);
+    if (next >= 0) put(b + 1);
     block = next;
     __syncthreads();
   }
@@ -232,18 +261,17 @@ __global__ __launch_bounds__(64 * W, RT * D > 384 ? 1 : 2) void tile_kernel(Call
   }
 }
 
-// Row tiles of a wave: the most whose sums, queries and logits (24, 40 or 88 registers each) leave two waves a SIMD (for
-// heads of 256: one), for each operand read from LDS feeds that many products.
-constexpr int TILE_WAVES = 4;
+// Row tiles of a wave. Heads of 128: two (535 us for 8192 tokens; three 532, one more block of work in the last
+// workgroup). Heads of 64 one (three sequences of 12000 tokens and 1500 rows of 8 heads over one: 95 us; two 96, with
+// half the workgroups for short calls); heads of 256 one, two spill.
 template <int D>
-constexpr int ROW_TILES = D == 64 ? 4 : D == 128 ? 3 : 2;
-int tile_rows(int dim) { return 16 * TILE_WAVES * (dim == 64 ? ROW_TILES<64> : dim == 128 ? ROW_TILES<128> : ROW_TILES<256>); }
+constexpr int ROW_TILES = D == 128 ? 2 : 1;
+int tile_rows(int dim) { return 128 * (dim == 128 ? ROW_TILES<128> : ROW_TILES<64>); }
 
 template <int D, int FMT, int DT>
 static void launch(const Call &c, const Pool &pool, const Rows &rows, int tiles, uint32_t total, hipStream_t st) {
-  constexpr int RT = ROW_TILES<D>, W = TILE_WAVES;
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_kernel<D, FMT, DT, RT, W>), dim3(total), dim3(64 * W), 2 * 16 * (D / 64) * 1024, st, c,
-                     pool, rows, tiles);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_kernel<D, FMT, DT, ROW_TILES<D>>), dim3(total), dim3(512), 2 * 16 * (D / 64) * 1024, st, c, pool,
+                     rows, tiles);
 }
 void launch_tile(const Call &c, const Pool &pool, const Rows &rows, int format, int dtype, int tiles, uint32_t total, hipStream_t st) {
 #define ISHZ_TILE_D(F, T)                                               \

@@ -9,13 +9,15 @@ output projection.
 
 A sequence's blocks stand in its row of a table, anywhere in the pool (`new_cache`). Functions return None when
 the library declines a shape or dtype; every check happens before a launch, and none waits for the GPU.
+
+Calls whose arguments fit as they are go through `_bind` (csrc/python/bind.cpp); what is below makes the others.
 """
 import math
 from typing import NamedTuple
 
 import torch
 
-from . import _lib
+from . import _bind, _lib
 from ._torch import DTYPES, ptr, require_cuda, stream
 
 BLOCK = 64
@@ -117,6 +119,9 @@ def _batch(b):
 def norm_rope(q, k, positions=None, turns=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, factor=1.0):
     """(q, k) [rows, heads, dim] normed over each head (where a weight is given) and turned by their positions
     (where `turns` is), computed in fp32 and rounded once to their dtype; None if declined."""
+    out = _bind.norm_rope(q, k, positions, turns, q_weight, k_weight, eps, interleaved, factor)
+    if out is not NotImplemented:
+        return out
     require_cuda(q, k, positions, turns, q_weight, k_weight)
     q, q_row, q_head = _heads(q, "q")
     k, k_row, k_head = _heads(k, "k")
@@ -139,6 +144,9 @@ def append(k, v, cache, batch, q=None, positions=None, turns=None, q_weight=None
     """Writes k and v [rows, heads, dim] behind what the batch's sequences hold, k normed and turned first as in
     `norm_rope` where asked. Returns q [rows, q heads, dim] normed and turned (True where there is no q); None if
     declined."""
+    out = _bind.append(k, v, cache, batch, q, positions, turns, q_weight, k_weight, eps, interleaved, factor)
+    if out is not NotImplemented:
+        return out
     require_cuda(k, v, q, positions, turns, q_weight, k_weight)
     pointers = _cache(cache)
     heads, dim = pointers[6:]
@@ -168,6 +176,9 @@ def append(k, v, cache, batch, q=None, positions=None, turns=None, q_weight=None
 def read(cache, batch, tail=None, dtype=torch.float16):
     """(k, v) [sequences, tail, heads, dim]: the last `tail` tokens (None: max_length) of each sequence, zeros where
     it has fewer; None if declined."""
+    out = _bind.read(cache, batch, tail, dtype)
+    if out is not NotImplemented:
+        return out
     pointers = _cache(cache)
     heads, dim = pointers[6:]
     table, width, lengths, _, sequences = _batch(batch)
@@ -185,6 +196,9 @@ def attend(q, cache, batch, scale=None, causal=True, window=0):
     """[rows, q heads, dim]: attention of the batch's rows over their sequences' tokens in the cache, weights
     softmax(scale q K^T) (`scale` None: dim ** -0.5). Causal: a row sees the tokens up to its own (`window` > 0: the
     last `window` of them); else all of its sequence's. A row that sees none gives zeros. None if declined."""
+    out = _bind.attend(q, cache, batch, scale, causal, window)
+    if out is not NotImplemented:
+        return out
     require_cuda(q)
     pointers = _cache(cache)
     heads, dim = pointers[6:]

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from ishizuki_amd import _lib, attention
+from ishizuki_amd import _bind, _lib, attention
 
 P = ctypes.c_void_p(4096)
 POOL = dict(k=P, v=P, ks=P, vs=P, format=0, blocks=4, heads=2, dim=128)
@@ -177,3 +177,13 @@ def test_strides_are_passed_and_odd_ones_copied(library):
     attention.attend(odd, cache, batch())
     args = library.calls[-1][1]
     assert args[0] % 16 == 0 and args[1:3] == (128, 64)
+
+
+def test_binding_leaves_what_does_not_fit():
+    """Without a GPU nothing fits: the compiled calls hand every call over, and raise nothing."""
+    x = torch.zeros(3, 2, 64, dtype=torch.float16)
+    cache = attention.new_cache(2, 2, 64, device="cpu")
+    for out in (_bind.norm_rope(x, x, None, None, None, None, 1e-6, False, 1.0), _bind.norm_rope(x), _bind.norm_rope(*[None] * 9),
+                _bind.attend(x, cache, batch(), None, True, 0), _bind.attend("q", (), 3, None, True, 0), _bind.read(cache, batch(), -1, torch.float16),
+                _bind.append(x, x, cache, batch(), None, None, None, None, None, 1e-6, False, 1.0), _bind.append()):
+        assert out is NotImplemented

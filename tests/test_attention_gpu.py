@@ -520,3 +520,49 @@ def test_declined():
     assert attention.read(cache, batch) is None and attention.norm_rope(x, x) is None
     cache = attention.new_cache(2, 1, 64, device=DEV)
     assert attention.attend(torch.zeros(1, 1, 64, device=DEV), cache, batch) is None
+
+
+class _None:
+    """Hands every call over to attention.py."""
+
+    def __getattr__(self, name):
+        return lambda *args: NotImplemented
+
+
+def test_binding_and_python_calls_agree(monkeypatch):
+    """The compiled calls take what fits, on the current stream, and give the bits of the calls made in Python; what does not
+    fit (copies of odd strides, refusals, declines) is the same through either."""
+    heads, kv, dim = 6, 2, 128
+    batch, blocks = make_batch([100, 40], [2, 3], seed=4)
+    first = gpu(random_cache(blocks, kv, dim, E4M3, seed=6))
+    qkv = normal(3, 5, heads + 2 * kv, dim, dtype=BF16).to(DEV)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv], qkv[:, heads + kv:]
+    table, positions, w = attention.turns(dim, device=DEV), i32(98, 99, 37, 38, 39).to(DEV), torch.full((dim,), 1.5, device=DEV)
+    odd = torch.zeros(5, heads, dim + 1, dtype=BF16, device=DEV)[..., 1:]
+    odd.copy_(q)
+
+    def calls():
+        cache = attention.Cache(*(t.clone() for t in first))
+        got = [*attention.norm_rope(q, k, positions, table, w, w, interleaved=True, factor=0.5), *attention.norm_rope(q, k),
+               attention.append(k, v, cache, batch, q=q, positions=positions, turns=table, q_weight=w, k_weight=w, eps=1e-5),
+               attention.attend(q, cache, batch, window=9), attention.attend(odd, cache, batch, scale=1),
+               attention.attend(q, cache, batch, causal=False), *attention.read(cache, batch, tail=70, dtype=F32), *attention.read(cache, batch)]
+        assert attention.append(k, v, cache, batch) is True
+        assert attention.attend(q.float(), cache, batch) is None
+        with pytest.raises(ValueError):
+            attention.attend(q[..., :64], cache, batch)
+        with pytest.raises(ValueError):
+            attention.norm_rope(q, k, positions[:3], table)
+        return got + [t.view(INT8) if t.dtype is E4M3 else t for t in cache]
+
+    assert attention._bind.attend(q, first, batch, None, True, 0) is not NotImplemented
+    assert attention._bind.read(first, batch, None, F16) is not NotImplemented
+    assert attention._bind.norm_rope(q, k, positions, table, w, w, 1e-6, False, 1.0) is not NotImplemented
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        compiled = calls()
+    torch.cuda.current_stream().wait_stream(side)
+    monkeypatch.setattr(attention, "_bind", _None())
+    for a, b in zip(compiled, calls(), strict=True):
+        assert torch.equal(a, b)

@@ -1,9 +1,21 @@
 // What the attention kernels share: the 8-bit cache's geometry and codes, the call's rows, per-head
 // norms and the position rotation.
 #pragma once
+#include <utility>
+
 #include "common.h"
 
 namespace attn {
+// f(0) .. f(N - 1) with constants, for bodies too long for the unroller's limit.
+template <class F, int... I>
+DEV void unrolled(std::integer_sequence<int, I...>, F &&f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+DEV void unrolled(F &&f) {
+  unrolled(std::make_integer_sequence<int, N>{}, f);
+}
+
 constexpr int BLOCK = ISHZ_KV_BLOCK;  // tokens that share a scale, for each head
 
 // The pool: codes of keys [blocks][heads][64][dim] and of values [blocks][heads][dim][64], their scales
@@ -151,12 +163,18 @@ DEV void unit_angles(const Turn &t, int u, int32_t position, float *c, float *s)
 }
 // x: the unit's sixteen values, in place.
 DEV void unit_turn(bool interleaved, const float *c, const float *s, float *x) {
+  // values chosen, not places: a place chosen at run time would put x into memory
+  float p[8], q[8];
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const float a = interleaved ? x[2 * i] : x[i], b = interleaved ? x[2 * i + 1] : x[8 + i];
-    const float p = a * c[i] - b * s[i], q = b * c[i] + a * s[i];
-    if (interleaved) x[2 * i] = p, x[2 * i + 1] = q;
-    else x[i] = p, x[8 + i] = q;
+    const float a0 = x[2 * i], a1 = x[i], b0 = x[2 * i + 1], b1 = x[8 + i];
+    const float a = interleaved ? a0 : a1, b = interleaved ? b0 : b1;
+    p[i] = a * c[i] - b * s[i], q[i] = b * c[i] + a * s[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const float y0 = i % 2 ? q[i / 2] : p[i / 2], y1 = i < 8 ? p[i % 8] : q[i % 8];
+    x[i] = interleaved ? y0 : y1;
   }
 }
 // Sum over the head's U = dim / 16 lanes (4, 8 or 16).
@@ -168,15 +186,15 @@ DEV float head_sum(float v) {
   if (U >= 16) v += ISHZ_DPP(v, 0x140);
   return v;
 }
-// Norms the unit's sixteen values in place; every lane of the head calls it. w: the head's weight.
+// Norms the unit's sixteen values in place; every lane of the head calls it. w: their weights.
 template <int U>
-DEV void unit_norm(float *x, const float *w, int ca, int cb, float eps) {
+DEV void unit_norm(float *x, const float *w, float eps) {
   float sum = 0;
 #pragma unroll
   for (int i = 0; i < 16; i++) sum += x[i] * x[i];
   const float r = 1.0f / sqrtf(head_sum<U>(sum) * (1.0f / (16 * U)) + eps);
 #pragma unroll
-  for (int i = 0; i < 16; i++) x[i] *= r * w[i < 8 ? ca + i : cb + i - 8];
+  for (int i = 0; i < 16; i++) x[i] *= r * w[i];
 }
 
 // ---------------------------------------------------------------- attention

@@ -13,38 +13,61 @@ struct Heads {
   void *out;            // [rows][heads][dim], or null
 };
 
-// Loads unit u of head h of a row, normed and turned. c, s: the unit's angles (u < rot / 16).
-template <int DT, int U>
-DEV void load_unit(const Heads &g, const Turn &t, float eps, int row, int h, int u, const float *c, const float *s, float *x) {
-  int ca, cb;
-  unit_chunks(u, t.rot, t.interleaved, &ca, &cb);
-  const size_t at = (size_t)(row * g.row + h * g.head);
-  load8<DT>(g.x, at + ca, x);
-  load8<DT>(g.x, at + cb, x + 8);
-  if (g.weight) unit_norm<U>(x, g.weight, ca, cb, eps);
-  if (u < t.rot / 16) unit_turn(t.interleaved, c, s, x);
-}
+// A unit's sixteen values as they are loaded.
+template <int DT>
+struct Raw {
+  u4 v[DT == ISHZ_DT_F32 ? 4 : 2];
+  DEV void load(const void *x, size_t at, int ca, int cb) {
+    constexpr int H = DT == ISHZ_DT_F32 ? 2 : 1, Z = DT == ISHZ_DT_F32 ? 4 : 2;
+#pragma unroll
+    for (int i = 0; i < H; i++) {
+      v[i] = *(const u4 *)((const uint8_t *)x + (at + ca) * Z + 16 * i);
+      v[H + i] = *(const u4 *)((const uint8_t *)x + (at + cb) * Z + 16 * i);
+    }
+  }
+  DEV void widen(float *x) const {
+    load8<DT>(v, 0, x);
+    load8<DT>(v, 8, x + 8);
+  }
+};
 
-// One wave's share of one row: part of `parts`, 64 / U heads at a time, over q's heads and then k's.
+// One wave's share of one row: part of `parts`, 64 / U heads at a time, over q's heads and then k's. The next heads' values
+// are on their way while these are worked on: 4096 rows of 28 heads of 256 in fp16 take 24.4 us without that.
 template <int DT, int U>
 DEV void turn_row(const Heads &q, const Heads &k, const Turn &t, float eps, int row, int part, int parts) {
   constexpr int W = 64 / U;
-  const int lane = threadIdx.x & 63, u = lane % U, total = q.heads + k.heads;
-  float c[8], s[8];
-  if (u < t.rot / 16) unit_angles(t, u, t.positions[row], c, s);
+  const int lane = threadIdx.x & 63, u = lane % U, gq = (q.heads + W - 1) / W, groups = gq + (k.heads + W - 1) / W;
   int ca, cb;
   unit_chunks(u, t.rot, t.interleaved, &ca, &cb);
-  for (int h0 = part * W; h0 < total; h0 += parts * W) {
-    const int h = h0 + lane / U, hc = min(h, total - 1);
-    const bool first = hc < q.heads;
-    const Heads &g = first ? q : k;
-    const int hh = first ? hc : hc - q.heads;
+  const auto load = [&](int g, Raw<DT> &x) {
+    const Heads &y = g < gq ? q : k;
+    const int h = min((g < gq ? g : g - gq) * W + lane / U, y.heads - 1);
+    x.load(y.x, (size_t)(row * y.row + h * y.head), ca, cb);
+  };
+  if (part >= groups) return;
+  Raw<DT> next;
+  load(part, next);
+  float c[8], s[8], w[16];
+  if (u < t.rot / 16) unit_angles(t, u, t.positions[row], c, s);
+  int held = -1;  // whose weight w is: 0 q's, 1 k's
+  for (int g = part; g < groups; g += parts) {
     float x[16];
-    load_unit<DT, U>(g, t, eps, row, hh, u, c, s, x);
-    if (h < total) {
-      const size_t to = ((size_t)row * g.heads + hh) * (16 * U);
-      store8<DT>(g.out, to + ca, x);
-      store8<DT>(g.out, to + cb, x + 8);
+    next.widen(x);
+    if (g + parts < groups) load(g + parts, next);
+    const int whose = g >= gq;
+    const Heads &y = whose ? k : q;
+    if (whose != held && y.weight) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) w[i] = y.weight[i < 8 ? ca + i : cb + i - 8];
+    }
+    held = whose;
+    if (y.weight) unit_norm<U>(x, w, eps);
+    if (u < t.rot / 16) unit_turn(t.interleaved, c, s, x);
+    const int h = (whose ? g - gq : g) * W + lane / U;
+    if (h < y.heads) {
+      const size_t to = ((size_t)row * y.heads + h) * (16 * U);
+      store8<DT>(y.out, to + ca, x);
+      store8<DT>(y.out, to + cb, x + 8);
     }
   }
 }
@@ -64,18 +87,39 @@ DEV uint32_t regrow4(uint32_t c, float down) {
   return encode4<FMT>(v[0] * down, v[1] * down, v[2] * down, v[3] * down);
 }
 
-// A workgroup per (sequence, block that its new rows reach, head, keys or values) owns that block's codes and
-// scale, so the scale is the exact maximum over its new tokens without a second pass or atomics; workgroups past
-// those turn q's heads, four rows each.
+// The block's scale for new tokens of largest magnitude `most` (bits) from slot s0 on, and by which power of two its older
+// codes go down. 2^-126 keeps it a normal number; a NaN or an infinity among the tokens makes it NaN, and so what is read
+// of this block and head, rather than being dropped. A partly filled block keeps its scale, or grows it by the least power
+// of two that holds the new tokens: its old codes are then rounded at most once for each doubling, and all those
+// roundings together stay below one step.
+template <int FMT>
+DEV float next_scale(uint32_t most, int s0, float old, int *grow) {
+  const float amax = __builtin_bit_cast(float, most);
+  *grow = 0;
+  if (most >= 0x7f800000u) return __builtin_nanf("");
+  if (s0 == 0) return fmaxf(amax / LIMIT<FMT>, 0x1p-126f);
+  const float scale = old < 0x1p-126f ? 0x1p-126f : old, held = LIMIT<FMT> * scale;
+  if (!(amax > held)) return scale;
+  int ea, eb;
+  const float ma = frexpf(amax, &ea), mb = frexpf(held, &eb);
+  *grow = ea - eb + (ma > mb);
+  return ldexpf(scale, *grow);
+}
+
+// A workgroup per (sequence, block that its new rows reach, head, keys or values) owns that block's codes and scale, so
+// the scale is the exact maximum over its new tokens without a second pass or atomics: the tokens stay in registers
+// meanwhile. Of keys a thread has units of a token (the norm and the rotation go over the head); of values 4 tokens of 8
+// dims, which are whole words of the block's rows of tokens: nothing is turned in LDS. Workgroups past those turn q's
+// heads, `waves` waves a row.
 template <int DT, int U, int FMT>
 __global__ __launch_bounds__(256) void append_kernel(Heads k, Heads v, Heads q, Turn t, float eps, Pool pool, Rows rows,
-                                                     int reach, int writers) {
-  constexpr int D = 16 * U, N = U / 4, PITCH = BLOCK + 16;
+                                                     int reach, int writers, int waves) {
+  constexpr int D = 16 * U, N = U / 4, G = U <= 8 ? 1 : 2;
   __shared__ uint32_t scratch[4];
-  __shared__ __attribute__((aligned(16))) uint8_t turned[D * PITCH];
+  const int tid = threadIdx.x;
   if ((int)blockIdx.x >= writers) {
-    const int row = (blockIdx.x - writers) * 4 + wave_id();
-    if (row < rows.rows) turn_row<DT, U>(q, Heads{}, t, eps, row, 0, 1);
+    const int wave = wave_id(), row = (blockIdx.x - writers) * (4 / waves) + wave / waves;
+    if (row < rows.rows) turn_row<DT, U>(q, Heads{}, t, eps, row, wave % waves, waves);
     return;
   }
   int id = blockIdx.x;
@@ -91,116 +135,119 @@ __global__ __launch_bounds__(256) void append_kernel(Heads k, Heads v, Heads q, 
   if (lo >= hi) return;
   const int block = rows.block(seq, jb, pool.blocks);
   if (block < 0) return;
-  const int s0 = lo - jb * BLOCK, s1 = hi - jb * BLOCK;
-  const Heads &g = values ? v : k;
-  const Turn none = {nullptr, nullptr, 0, 0, 1.0f};
-  const Turn &turn = values ? none : t;
-
-  float x[N][16];
-  uint32_t most = 0;
-#pragma unroll
-  for (int m = 0; m < N; m++) {
-    if (256 * m / U >= s1 - s0) break;
-    const int unit = threadIdx.x + 256 * m, u = unit % U;
-    const int row = row0 + lo - start + min(unit / U, s1 - s0 - 1);
-    float c[8], s[8];
-    if (u < turn.rot / 16) unit_angles(turn, u, turn.positions[row], c, s);
-    load_unit<DT, U>(g, turn, eps, row, head, u, c, s, x[m]);
-#pragma unroll
-    for (int i = 0; i < 16; i++) most = max(most, __builtin_bit_cast(uint32_t, x[m][i]) & 0x7fffffffu);
-  }
+  const int s0 = lo - jb * BLOCK, s1 = hi - jb * BLOCK, row_of = row0 + jb * BLOCK - start;  // of slot 0
   float *const scale_at = (values ? pool.vs : pool.ks) + pool.scale(block, head);
   const float old = *scale_at;
-  most = block_absmax(most, scratch);
-
-  // The block's scale. 2^-126 keeps it a normal number; a NaN or an infinity among the tokens makes it NaN, and so
-  // what is read of this block and head, rather than being dropped.
-  const float amax = __builtin_bit_cast(float, most);
-  float scale, down = 1.0f;
-  int grow = 0;
-  if (most >= 0x7f800000u) {
-    scale = __builtin_nanf("");
-  } else if (s0 == 0) {
-    scale = fmaxf(amax / LIMIT<FMT>, 0x1p-126f);
-  } else {
-    // A partly filled block keeps its scale, or grows it by the least power of two that holds the new tokens: its old
-    // codes are then rounded at most once for each doubling, and all those roundings together stay below one step.
-    scale = old < 0x1p-126f ? 0x1p-126f : old;
-    const float held = LIMIT<FMT> * scale;
-    if (amax > held) {
-      int ea, eb;
-      const float ma = frexpf(amax, &ea), mb = frexpf(held, &eb);
-      grow = ea - eb + (ma > mb);
-      scale = ldexpf(scale, grow);
-      down = ldexpf(1.0f, -grow);
-    }
-  }
-  if (threadIdx.x == 0) *scale_at = scale;
-  const float up = scale == scale ? 1.0f / scale : 0.0f;
-  const bool dead = scale != scale;
-
   uint8_t *const tile = (values ? pool.v : pool.k) + pool.tile(block, head);
-#pragma unroll
-  for (int m = 0; m < N; m++) {
-    const int unit = threadIdx.x + 256 * m, u = unit % U, slot = s0 + unit / U;
-    if (slot >= s1) continue;
-    int ca, cb;
-    unit_chunks(u, turn.rot, turn.interleaved, &ca, &cb);
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      w[i] = dead ? 0 : encode4<FMT>(x[m][4 * i] * up, x[m][4 * i + 1] * up, x[m][4 * i + 2] * up, x[m][4 * i + 3] * up);
-    if (!values) {
-      *(u2 *)(tile + slot * D + ca) = u2{w[0], w[1]};
-      *(u2 *)(tile + slot * D + cb) = u2{w[2], w[3]};
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; i++) turned[((i < 8 ? ca + i : cb + i - 8)) * PITCH + slot] = (uint8_t)(w[i / 4] >> 8 * (i % 4));
-    }
-  }
+  uint32_t most = 0;
+  const auto larger = [&](float x) { most = max(most, __builtin_bit_cast(uint32_t, x) & 0x7fffffffu); };
+
   if (!values) {
-    if (grow > 0)
-      for (int i = threadIdx.x; i < s0 * D / 16; i += 256) {
+    const int u = tid % U;
+    int ca, cb;
+    unit_chunks(u, t.rot, t.interleaved, &ca, &cb);
+    float x[N][16], w[16];
+    if (k.weight) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) w[i] = k.weight[i < 8 ? ca + i : cb + i - 8];
+    }
+    Raw<DT> raw[N];
+#pragma unroll
+    for (int m = 0; m < N; m++)  // slots past the last read the last one's token again: whole heads take part in a norm
+      raw[m].load(k.x, (size_t)((int64_t)(row_of + min(s0 + (tid + 256 * m) / U, s1 - 1)) * k.row + head * k.head), ca, cb);
+    unrolled<N>([&](auto m) __attribute__((always_inline)) {
+      raw[m].widen(x[m]);
+      if (256 * m / U < s1 - s0) {  // the same for the whole workgroup
+        if (k.weight) unit_norm<U>(x[m], w, eps);
+        if (u < t.rot / 16) {
+          float c[8], s[8];
+          unit_angles(t, u, t.positions[row_of + min(s0 + (tid + 256 * m) / U, s1 - 1)], c, s);
+          unit_turn(t.interleaved, c, s, x[m]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; i++) larger(x[m][i]);
+    });
+    int grow;
+    const float scale = next_scale<FMT>(block_absmax(most, scratch), s0, old, &grow), up = 1.0f / scale;
+    if (tid == 0) *scale_at = scale;
+#pragma unroll
+    for (int m = 0; m < N; m++) {
+      const int slot = s0 + (tid + 256 * m) / U;
+      if (slot >= s1) continue;
+      uint32_t code[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        code[i] = scale != scale ? 0 : encode4<FMT>(x[m][4 * i] * up, x[m][4 * i + 1] * up, x[m][4 * i + 2] * up, x[m][4 * i + 3] * up);
+      *(u2 *)(tile + slot * D + ca) = u2{code[0], code[1]};
+      *(u2 *)(tile + slot * D + cb) = u2{code[2], code[3]};
+    }
+    if (grow > 0) {
+      const float down = ldexpf(1.0f, -grow);
+      for (int i = tid; i < s0 * D / 16; i += 256) {
         u4 o = *(u4 *)(tile + 16 * i);
 #pragma unroll
         for (int e = 0; e < 4; e++) o[e] = regrow4<FMT>(o[e], down);
         *(u4 *)(tile + 16 * i) = o;
       }
-    return;
-  }
-  __syncthreads();
-  if (s0 == 0 && s1 == BLOCK) {
-    for (int i = threadIdx.x; i < D * 4; i += 256)
-      *(u4 *)(tile + 16 * i) = *(const u4 *)(turned + i / 4 * PITCH + 16 * (i % 4));
-    return;
-  }
-  // Four tokens of a value at a time, from the first that changes.
-  const int w0 = grow > 0 ? 0 : s0 / 4, words = (s1 + 3) / 4 - w0;
-  for (int i = threadIdx.x; i < D * words; i += 256) {
-    const int d = i / words, w = w0 + i % words;
-    uint32_t *const at = (uint32_t *)(tile + d * BLOCK + 4 * w);
-    const uint32_t fresh = *(const uint32_t *)(turned + d * PITCH + 4 * w);
-    if (4 * w >= s0 && 4 * w + 4 <= s1) {
-      *at = fresh;
-      continue;
     }
-    const uint32_t was = *at, kept = grow > 0 ? regrow4<FMT>(was, down) : was;
-    uint32_t o = 0;
+    return;
+  }
+
+  const int first = 4 * (tid % 16), dims = 8 * (tid / 16);  // this thread's slots and dims (of each 128)
+  const bool mine = dims < D;
+  float x[G][4][8];
 #pragma unroll
-    for (int b = 0; b < 4; b++) {
-      const int slot = 4 * w + b;
-      o |= (slot < s0 ? kept : slot < s1 ? fresh : was) & (255u << 8 * b);
+  for (int g = 0; g < G; g++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int slot = first + i;
+      if (mine && slot >= s0 && slot < s1)
+        load8<DT>(v.x, (size_t)((int64_t)(row_of + slot) * v.row + head * v.head) + dims + 128 * g, x[g][i]);
+      else
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[g][i][e] = 0;
     }
-    *at = o;
-  }
+#pragma unroll
+  for (int g = 0; g < G; g++)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) larger(x[g][i][e]);
+  int grow;
+  const float scale = next_scale<FMT>(block_absmax(most, scratch), s0, old, &grow), up = 1.0f / scale, down = ldexpf(1.0f, -grow);
+  if (tid == 0) *scale_at = scale;
+  // words that hold none of the new tokens are left alone, or lose steps where the scale grew
+  if (!mine || first >= s1 || (first + 4 <= s0 && grow <= 0)) return;
+  uint32_t fresh = 0;  // the bytes of new tokens
+#pragma unroll
+  for (int i = 0; i < 4; i++) fresh |= first + i >= s0 && first + i < s1 ? 255u << 8 * i : 0;
+#pragma unroll
+  for (int g = 0; g < G; g++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      uint32_t *const at = (uint32_t *)(tile + (dims + 128 * g + e) * BLOCK + first);
+      uint32_t code = scale != scale ? 0 : encode4<FMT>(x[g][0][e] * up, x[g][1][e] * up, x[g][2][e] * up, x[g][3][e] * up);
+      if (fresh != ~0u) {
+        const uint32_t was = *at;
+        // tokens past s1 in a word are none of the sequence's: what is made of them does not matter, but they stay
+        uint32_t past = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) past |= first + i >= s1 ? 255u << 8 * i : 0;
+        const uint32_t kept = grow > 0 ? (regrow4<FMT>(was, down) & ~past) | (was & past) : was;
+        code = (code & fresh) | (kept & ~fresh);
+      }
+      *at = code;
+    }
 }
 
 // ---------------------------------------------------------------- reading
-// A workgroup per (sequence, block that holds some of its last `tail` tokens, head, keys or values).
-template <int DT, int FMT>
+// A workgroup per (sequence, block that holds some of its last `tail` tokens, head, keys or values). A thread has 8 dims of a
+// token of keys at a time, 4 tokens of 8 dims of values: loads of words of the block's rows, stores of 16 bytes.
+template <int DT, int D, int FMT>
 __global__ __launch_bounds__(256) void read_kernel(Pool pool, Rows rows, int tail, int reach, void *k_out, void *v_out) {
-  __shared__ __attribute__((aligned(16))) uint8_t turned[BLOCK * (256 + 16)];
-  const int D = pool.dim, pitch = D + 16;
+  constexpr int PER = D / 8, G = D == 256 ? 2 : 1;
+  const int tid = threadIdx.x;
   int id = blockIdx.x;
   const int head = id % pool.heads;
   id /= pool.heads;
@@ -208,31 +255,49 @@ __global__ __launch_bounds__(256) void read_kernel(Pool pool, Rows rows, int tai
   id >>= 1;
   const int j = id % reach, seq = id / reach;
   const int length = rows.length(seq), p0 = length - tail, jb = (p0 >> 6) + j;
-  const int lo = max(p0, jb * BLOCK), hi = min(length, jb * BLOCK + BLOCK);
-  if (lo >= hi) return;
+  const int s0 = max(p0 - jb * BLOCK, 0), s1 = min(length - jb * BLOCK, BLOCK);
+  if (s0 >= s1) return;
   const int block = rows.block(seq, jb, pool.blocks);
   const float scale = block < 0 ? 0.0f : (values ? pool.vs : pool.ks)[pool.scale(block, head)];
   const uint8_t *const tile = (values ? pool.v : pool.k) + pool.tile(max(block, 0), head);
-  if (values && block >= 0) {
-    for (int i = threadIdx.x; i < D * 4; i += 256) {
-      const u4 c = *(const u4 *)(tile + 16 * i);
+  // of slot 0 and dim 0
+  const int64_t at = (((int64_t)seq * tail + (jb * BLOCK - p0)) * pool.heads + head) * D;
+  const int64_t step = (int64_t)pool.heads * D;
+  if (!values) {
+    const int d = 8 * (tid % PER);
+    u2 c[D / 32];
 #pragma unroll
-      for (int e = 0; e < 16; e++) turned[(16 * (i % 4) + e) * pitch + i / 4] = (uint8_t)(c[e / 4] >> 8 * (e % 4));
+    for (int i = 0; i < D / 32; i++) {
+      const int slot = tid / PER + i * (256 / PER);
+      c[i] = block >= 0 && slot >= s0 && slot < s1 ? *(const u2 *)(tile + slot * D + d) : u2{0, 0};
     }
-    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+      const int slot = tid / PER + i * (256 / PER);
+      if (slot < s0 || slot >= s1) continue;
+      const f4 a = decode4f<FMT>(c[i].x) * scale, b = decode4f<FMT>(c[i].y) * scale;
+      const float o[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      store8<DT>(k_out, (size_t)(at + slot * step + d), o);
+    }
+    return;
   }
-  void *const out = values ? v_out : k_out;
-  const int per = D / 8;
-  for (int i = threadIdx.x; i < (hi - lo) * per; i += 256) {
-    const int p = lo + i / per, slot = p - jb * BLOCK, d = i % per * 8;
-    float o[8] = {};
-    if (block >= 0) {
-      const u2 c = values ? *(const u2 *)(turned + slot * pitch + d) : *(const u2 *)(tile + slot * D + d);
-      const f4 a = decode4f<FMT>(c.x), b = decode4f<FMT>(c.y);
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[e] = a[e] * scale, o[4 + e] = b[e] * scale;
+  for (int g = 0; g < G; g++) {
+    const int d = 8 * (tid % PER), first = 4 * (tid / PER) + 32 * g;
+    if (first >= BLOCK) return;
+    uint32_t c[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) c[e] = block >= 0 ? *(const uint32_t *)(tile + (d + e) * BLOCK + first) : 0;
+    f4 x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = decode4f<FMT>(c[e]) * scale;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int slot = first + i;
+      if (slot < s0 || slot >= s1) continue;
+      const float o[8] = {x[0][i], x[1][i], x[2][i], x[3][i], x[4][i], x[5][i], x[6][i], x[7][i]};
+      store8<DT>(v_out, (size_t)(at + slot * step + d), o);
     }
-    store8<DT>(out, (((size_t)seq * tail + (p - p0)) * pool.heads + head) * D + d, o);
   }
 }
 
@@ -337,7 +402,8 @@ extern "C" int ishz_kv_append(const void *k, int64_t k_row, int64_t k_head, cons
   // max_rows rows that start anywhere in a block reach this many.
   max_rows = std::min(max_rows, rows);
   const int reach = max_rows > 0 ? (max_rows + BLOCK - 2) / BLOCK + 1 : 0;
-  const int64_t writers = (int64_t)sequences * reach * 2 * heads, turners = q_heads ? (rows + 3) / 4 : 0;
+  const int64_t writers = (int64_t)sequences * reach * 2 * heads, waves = rows >= 2048 ? 1 : 4;  // as for ishz_norm_rope
+  const int64_t turners = q_heads ? (rows + 4 / waves - 1) / (4 / waves) : 0;
   if (writers + turners > (1 << 24) - 1) return ishz::decline("more blocks than a launch holds");
   if (writers + turners == 0) return ISHZ_OK;
   const Heads gk = {k, k_row, k_head, heads, k_weight, nullptr}, gv = {v, v_row, v_head, heads, nullptr, nullptr};
@@ -347,7 +413,7 @@ extern "C" int ishz_kv_append(const void *k, int64_t k_row, int64_t k_head, cons
   const Rows r = {table, lengths, starts, sequences, width, rows};
   ISHZ_BY_FORMAT(format, ISHZ_BY_DTYPE(dtype, ISHZ_BY_DIM(dim, hipLaunchKernelGGL(
       HIP_KERNEL_NAME(append_kernel<DT, U, FMT>), dim3((uint32_t)(writers + turners)), dim3(256), 0, ishz::S(stream), gk, gv, gq,
-      t, eps, pool, r, reach, (int)writers))));
+      t, eps, pool, r, reach, (int)writers, (int)waves))));
   ISHZ_LAUNCH_CHECK("cache append launch");
   return ISHZ_OK;
 }
@@ -365,9 +431,9 @@ extern "C" int ishz_kv_read(const void *k_codes, const void *v_codes, const floa
   if (total > (1 << 24) - 1) return ishz::decline("more blocks than a launch holds");
   const Pool pool = {(uint8_t *)k_codes, (uint8_t *)v_codes, (float *)k_scale, (float *)v_scale, blocks, heads, dim};
   const Rows r = {table, lengths, nullptr, sequences, width, 0};
-  ISHZ_BY_FORMAT(format, ISHZ_BY_DTYPE(dtype, hipLaunchKernelGGL(HIP_KERNEL_NAME(read_kernel<DT, FMT>), dim3((uint32_t)total),
-                                                                 dim3(256), 0, ishz::S(stream), pool, r, tail, (int)reach,
-                                                                 k_out, v_out)));
+  ISHZ_BY_FORMAT(format, ISHZ_BY_DTYPE(dtype, ISHZ_BY_DIM(dim, hipLaunchKernelGGL(
+      HIP_KERNEL_NAME(read_kernel<DT, 16 * U, FMT>), dim3((uint32_t)total), dim3(256), 0, ishz::S(stream), pool, r, tail, (int)reach,
+      k_out, v_out))));
   ISHZ_LAUNCH_CHECK("cache read launch");
   return ISHZ_OK;
 }

@@ -109,14 +109,17 @@ DEV uint32_t narrow2(float a, float b) {
   if (DT == ISHZ_DT_F16) return (uint32_t)f2h(a) | (uint32_t)f2h(b) << 16;
   return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16;
 }
-template <int DT>
+template <int DT, bool PAST = false>  // PAST: past the caches
 DEV void store8(void *p, size_t i, const float *v) {
+  const auto put = [&](u4 x, u4 *at) {
+    if (PAST) __builtin_nontemporal_store(x, at);
+    else *at = x;
+  };
   if (DT == ISHZ_DT_F32) {
-    *(f4 *)((float *)p + i) = f4{v[0], v[1], v[2], v[3]};
-    *(f4 *)((float *)p + i + 4) = f4{v[4], v[5], v[6], v[7]};
+    put(__builtin_bit_cast(u4, (f4{v[0], v[1], v[2], v[3]})), (u4 *)((float *)p + i));
+    put(__builtin_bit_cast(u4, (f4{v[4], v[5], v[6], v[7]})), (u4 *)((float *)p + i + 4));
   } else {
-    *(u4 *)((uint16_t *)p + i) = u4{narrow2<DT>(v[0], v[1]), narrow2<DT>(v[2], v[3]), narrow2<DT>(v[4], v[5]),
-                                   narrow2<DT>(v[6], v[7])};
+    put(u4{narrow2<DT>(v[0], v[1]), narrow2<DT>(v[2], v[3]), narrow2<DT>(v[4], v[5]), narrow2<DT>(v[6], v[7])}, (u4 *)((uint16_t *)p + i));
   }
 }
 
@@ -238,9 +241,10 @@ DEV float load_query(const Call &c, int64_t row, int head, int quad, h8 *q) {
   return scale;
 }
 
-// tile_kernel (attn_tile.hip): packed rows of a workgroup, and its launch over `tiles` of them a sequence.
-int tile_rows(int dim);
-void launch_tile(const Call &c, const Pool &pool, const Rows &rows, int format, int dtype, int tiles, uint32_t total, hipStream_t st);
+// tile_kernel (attn_tile.hip) with 128 row_tiles packed rows to a workgroup (two only of heads of 128), `tiles` workgroups a
+// sequence, head and split.
+void launch_tile(const Call &c, const Pool &pool, const Rows &rows, int format, int dtype, int row_tiles, int tiles, uint32_t total,
+                 hipStream_t st);
 
 // What every call on the cache refuses (attn_cache.hip).
 int check_pool(const void *k, const void *v, const float *ks, const float *vs, int format, int blocks, int heads, int dim);

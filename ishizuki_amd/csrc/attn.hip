@@ -10,13 +10,13 @@ namespace attn {
 //   S^T [64 tokens x 16 rows] = K Q^T: the operand's row r of tile t is token 16 (r / 4) + 4 t + r % 4, so that a lane
 //   ends up with the weights of the 16 consecutive tokens 16 (lane / 16).. of row lane % 16;
 //   O^T [dim x 16 rows] += V^T P^T: those 16 weights are two operands as they are, against 16 consecutive bytes of V^T.
-// Neither codes nor weights pass through LDS, and each is read from memory once. The four waves of a workgroup take
-// every fourth block and are joined in LDS; splits of a long cache are joined by join_kernel.
-template <int D, int FMT, int DT, int RT>
-__global__ __launch_bounds__(256) void stream_kernel(Call c, Pool pool, Rows rows, int tiles) {
+// Neither codes nor weights pass through LDS, and each is read from memory once. The W waves of a workgroup take every
+// W-th block and are joined in LDS; splits of a long cache are joined by join_kernel.
+template <int D, int FMT, int DT, int RT, int W>
+__global__ __launch_bounds__(64 * W) void stream_kernel(Call c, Pool pool, Rows rows, int tiles) {
   constexpr int C = D / 64, V = D / 16, PITCH = D + 4;
-  __shared__ float joined[4 * 16 * PITCH];
-  __shared__ float wave_m[4][16], wave_l[4][16];
+  extern __shared__ __attribute__((aligned(16))) float joined[];  // [W][16][PITCH]
+  __shared__ float wave_m[W][16], wave_l[W][16];
   int id = blockIdx.x;
   const int kvh = id % pool.heads;
   id /= pool.heads;
@@ -56,8 +56,10 @@ __global__ __launch_bounds__(256) void stream_kernel(Call c, Pool pool, Rows row
 #pragma unroll
     for (int d = 0; d < V; d++) o[t][d] = f4{0, 0, 0, 0};
   }
-  for (int b = first + wave; b < stop; b += 4) {
-    const int block = __builtin_amdgcn_readfirstlane(rows.block(seq, b, pool.blocks));
+  int next = first + wave < stop ? rows.block(seq, first + wave, pool.blocks) : -1;
+  for (int b = first + wave; b < stop; b += W) {
+    const int block = __builtin_amdgcn_readfirstlane(next);
+    next = b + W < stop ? rows.block(seq, b + W, pool.blocks) : -1;
     if (block < 0) continue;
     const uint8_t *const kt = pool.k + pool.tile(block, kvh), *const vt = pool.v + pool.tile(block, kvh);
     const float ks = pool.ks[pool.scale(block, kvh)], vs = pool.vs[pool.scale(block, kvh)];
@@ -159,14 +161,16 @@ __global__ __launch_bounds__(256) void stream_kernel(Call c, Pool pool, Rows row
 #pragma unroll
     for (int d = 0; d < V; d++) *(f4 *)(joined + (wave * 16 + col) * PITCH + 16 * d + 4 * quad) = o[t][d];
     __syncthreads();
-    for (int x = threadIdx.x; x < 16 * (D / 8); x += 256) {
+    for (int x = threadIdx.x; x < 16 * (D / 8); x += 64 * W) {
       const int rr = x / (D / 8), d = x % (D / 8) * 8, r = r0 + 16 * t + rr;
       if (r >= packed) continue;
-      const float top = fmaxf(fmaxf(wave_m[0][rr], wave_m[1][rr]), fmaxf(wave_m[2][rr], wave_m[3][rr]));
+      float top = wave_m[0][rr];
+#pragma unroll
+      for (int w = 1; w < W; w++) top = fmaxf(top, wave_m[w][rr]);
       const float ref = top == -__builtin_inff() ? 0.0f : top;
       float acc[8] = {}, all = 0;
 #pragma unroll
-      for (int w = 0; w < 4; w++) {
+      for (int w = 0; w < W; w++) {
         const float f = __builtin_amdgcn_exp2f(wave_m[w][rr] - ref);
         all += f * wave_l[w][rr];
         const f4 a = *(const f4 *)(joined + (w * 16 + rr) * PITCH + d), a2 = *(const f4 *)(joined + (w * 16 + rr) * PITCH + d + 4);
@@ -188,48 +192,86 @@ __global__ __launch_bounds__(256) void stream_kernel(Call c, Pool pool, Rows row
   }
 }
 
-// Joins the splits of a row and head: D / 8 lanes each.
+// Joins the splits of a row and head, a wave: lane s has split s's maximum and sum (64 splits at most), then each lane
+// D / 64 of the values of all splits, eight of them on their way at a time.
 template <int D, int DT>
 __global__ __launch_bounds__(256) void join_kernel(Call c, const int32_t *starts, int sequences, int rows) {
-  const size_t at = (size_t)blockIdx.x * (256 / (D / 8)) + threadIdx.x / (D / 8);
-  const size_t total = (size_t)rows * c.heads;
+  constexpr int N = D / 64;
+  typedef float fn __attribute__((ext_vector_type(N)));
+  const int lane = threadIdx.x & 63;
+  const size_t at = (size_t)blockIdx.x * 4 + wave_id(), total = (size_t)rows * c.heads;
   const int64_t row = at / c.heads;
   if (row >= rows || row < starts[0] || row >= starts[sequences]) return;
-  const int d = threadIdx.x % (D / 8) * 8;
-  float top = -__builtin_inff();
-  for (int s = 0; s < c.splits; s++) top = fmaxf(top, c.ml[s * total + at].x);
-  const float ref = top == -__builtin_inff() ? 0.0f : top;
-  float acc[8] = {}, all = 0;
-  for (int s = 0; s < c.splits; s++) {
-    const float2 ml = c.ml[s * total + at];
-    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-    all += f * ml.y;
-    float x[8];
-    load8<ISHZ_DT_F32>(c.part, (s * total + at) * D + d, x);
+  const float2 ml = lane < c.splits ? c.ml[lane * total + at] : float2{-__builtin_inff(), 0.0f};
+  float top = ml.x;
+  top = fmaxf(top, ISHZ_DPP(top, 0xB1));
+  top = fmaxf(top, ISHZ_DPP(top, 0x4E));
+  top = fmaxf(top, ISHZ_DPP(top, 0x141));
+  top = fmaxf(top, ISHZ_DPP(top, 0x140));
+  top = fmaxf(top, lane_xor16(top));
+  top = fmaxf(top, lane_xor32(top));
+  const float f = __builtin_amdgcn_exp2f(ml.x - (top == -__builtin_inff() ? 0.0f : top));
+  const float all = group_sum<64>(f * ml.y);
+  const float *const part = c.part + at * D + lane * N;
+  float acc[N] = {};
+  for (int s0 = 0; s0 < c.splits; s0 += 8) {
+    fn x[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) acc[i] += f * x[i];
+    for (int i = 0; i < 8; i++) x[i] = *(const fn *)(part + min(s0 + i, c.splits - 1) * total * D);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float by = s0 + i < c.splits ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s0 + i)) : 0.0f;
+#pragma unroll
+      for (int e = 0; e < N; e++) acc[e] += by * x[i][e];
+    }
   }
   const float inv = all == 0 ? 0.0f : 1.0f / all;
 #pragma unroll
-  for (int i = 0; i < 8; i++) acc[i] *= inv;
-  store8<DT>(c.out, at * D + d, acc);
+  for (int e = 0; e < N; e++) acc[e] *= inv;
+  uint16_t *const out = (uint16_t *)c.out + at * D + lane * N;
+  if constexpr (N == 1) *out = (uint16_t)narrow2<DT>(acc[0], 0.0f);
+  else if constexpr (N == 2) *(uint32_t *)out = narrow2<DT>(acc[0], acc[1]);
+  else *(u2 *)out = u2{narrow2<DT>(acc[0], acc[1]), narrow2<DT>(acc[2], acc[3])};
 }
 
 // How a call is divided: packed rows to a workgroup, and splits of the cache.
 struct Plan {
-  int row_tiles, tiles, splits;  // row_tiles 0: tile_kernel
+  bool stream;  // stream_kernel, or tile_kernel
+  int row_tiles, tiles, splits, waves;
 };
 static Plan plan(int q_heads, int heads, int dim, int sequences, int max_rows, int max_length) {
   Plan p;
-  const int64_t packed = (int64_t)max_rows * (q_heads / heads);
-  p.row_tiles = packed <= 16 ? 1 : packed <= 32 ? 2 : 0;
-  const int per = p.row_tiles ? 16 * p.row_tiles : tile_rows(dim);
-  p.tiles = (int)((packed + per - 1) / per);
-  const int64_t groups = (int64_t)sequences * heads * p.tiles;
-  const int64_t blocks = ((int64_t)max_length + BLOCK - 1) / BLOCK;
-  const int64_t want = p.row_tiles ? 1024 : 512;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want + groups - 1) / std::max<int64_t>(groups, 1), (blocks + 3) / 4, 64}));
-  if (!p.row_tiles && groups * 2 > want) p.splits = 1;
+  const int64_t packed = (int64_t)max_rows * (q_heads / heads), blocks = ((int64_t)max_length + BLOCK - 1) / BLOCK;
+  const int64_t pairs = std::max<int64_t>((int64_t)sequences * heads, 1);
+  const auto tiles = [&](int per) { return (packed + per - 1) / per; };
+  // Sixteen packed rows or fewer stream; of heads of 256, whose codes take most of the registers, only while a wave has
+  // but a few blocks (64 blocks of 2 heads: 11.9 us, tiles 13.3; 256 of 32: 82 and 61). Up to 32 rows do of heads of 128
+  // (four sequences of 8191 tokens, 8 heads: 23.8 us, tiles 31.8; of 64 21.3 and 18.5, of 256 38 and 24.5).
+  p.stream = packed <= 16 ? dim < 256 || pairs * blocks < 1024 : packed <= 32 && dim == 128;
+  p.waves = 4;
+  int64_t splits;
+  if (p.stream) {
+    p.row_tiles = packed <= 16 ? 1 : 2;
+    p.tiles = (int)tiles(16 * p.row_tiles);
+    if (p.row_tiles == 1 && dim < 256 && blocks > 4 && blocks <= 16) {
+      p.waves = 8;  // two blocks a wave and one launch (13 blocks: 9.6 us; four waves, four splits and their join: 10.1)
+      splits = 1;
+    } else {
+      // Four workgroups a CU, and at most 32 blocks a wave's share of four, so that long sequences beside short ones end
+      // sooner (16 sequences of 12000 to 32768 tokens, 8 heads: 138 us, 141 without; 60000 of one: 32.5).
+      splits = std::min(std::max((1024 + pairs - 1) / pairs, blocks / 32), (blocks + 3) / 4);
+    }
+  } else {
+    // 256 rows a workgroup halve the decoding: for many (4096 tokens of 32 heads over 8: 150 us, 128 rows 185), or few rows
+    // over a long cache (512 over 16384: 148 and 158). Otherwise 128 rows end more evenly (2048 tokens: 59 us, 72).
+    const bool wide = dim == 128 && packed > 128 && (pairs * tiles(256) >= 512 || (blocks >= 128 && max_length >= 4 * (int64_t)max_rows));
+    p.row_tiles = wide ? 2 : 1;
+    p.tiles = (int)tiles(128 * p.row_tiles);
+    // A workgroup a CU, and at least six blocks each (128 rows over 4096 tokens: one split 83 us, eight 24; 512 tokens among
+    // themselves: one 17, two 23).
+    splits = std::min(256 / std::max<int64_t>(pairs * p.tiles, 1), blocks / 6);
+  }
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, 64));
   return p;
 }
 }  // namespace attn
@@ -264,22 +306,24 @@ extern "C" int ishz_kv_attend(const void *q, int64_t q_row, int64_t q_head, int 
   const Plan p = plan(q_heads, heads, dim, sequences, max_rows, max_length);
   const size_t need = p.splits == 1 ? 0 : (size_t)p.splits * rows * q_heads * (dim + 2) * 4;
   if (workspace_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 15)))) return ishz::einval("workspace too small");
-  const int64_t total = (int64_t)sequences * heads * p.tiles * p.splits, joins = ((int64_t)rows * q_heads + 256 / (dim / 8) - 1) / (256 / (dim / 8));
+  const int64_t total = (int64_t)sequences * heads * p.tiles * p.splits, joins = ((int64_t)rows * q_heads + 3) / 4;
   if (total > (1 << 24) - 1 || joins > (1 << 24) - 1) return ishz::decline("more rows than a launch holds");
   float *const part = (float *)workspace;
   const Call c = {q, q_row, q_head, out, q_heads, group, scale * 1.44269504088896341f, causal, window, p.splits, part,
                   (float2 *)(part + (need ? (size_t)p.splits * rows * q_heads * dim : 0))};
   const Pool pool = {(uint8_t *)k_codes, (uint8_t *)v_codes, (float *)k_scale, (float *)v_scale, blocks, heads, dim};
   const Rows r = {table, lengths, starts, sequences, width, rows};
-#define ISHZ_STREAM(D, F, T, RT)                                                                                         \
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(stream_kernel<D, F, T, RT>), dim3((uint32_t)total), dim3(256), 0, ishz::S(stream), c, pool, r, \
-                     p.tiles)
-#define ISHZ_STREAM_RT(D, F, T) if (p.row_tiles == 1) ISHZ_STREAM(D, F, T, 1); else ISHZ_STREAM(D, F, T, 2)
-#define ISHZ_STREAM_D(F, T)                          \
-  if (dim == 64) { ISHZ_STREAM_RT(64, F, T); }       \
-  else if (dim == 128) { ISHZ_STREAM_RT(128, F, T); } \
-  else { ISHZ_STREAM_RT(256, F, T); }
-  if (!p.row_tiles) launch_tile(c, pool, r, format, dtype, p.tiles, (uint32_t)total, ishz::S(stream));
+#define ISHZ_STREAM(D, F, T, RT, W)                                                                                      \
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(stream_kernel<D, F, T, RT, W>), dim3((uint32_t)total), dim3(64 * W),                 \
+                     W * 16 * (D + 4) * 4, ishz::S(stream), c, pool, r, p.tiles)
+#define ISHZ_STREAM_D(F, T)                                            \
+  if (dim == 64 && p.waves == 8) ISHZ_STREAM(64, F, T, 1, 8);          \
+  else if (dim == 64) ISHZ_STREAM(64, F, T, 1, 4);                     \
+  else if (dim == 256) ISHZ_STREAM(256, F, T, 1, 4);                   \
+  else if (p.waves == 8) ISHZ_STREAM(128, F, T, 1, 8);                 \
+  else if (p.row_tiles == 1) ISHZ_STREAM(128, F, T, 1, 4);             \
+  else ISHZ_STREAM(128, F, T, 2, 4)
+  if (!p.stream) launch_tile(c, pool, r, format, dtype, p.row_tiles, p.tiles, (uint32_t)total, ishz::S(stream));
   else if (format == ISHZ_KV_INT8) {
     if (dtype == ISHZ_DT_F16) { ISHZ_STREAM_D(ISHZ_KV_INT8, ISHZ_DT_F16); } else { ISHZ_STREAM_D(ISHZ_KV_INT8, ISHZ_DT_BF16); }
   } else {

@@ -34,15 +34,6 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(Call c, Pool pool, Rows ro
   const int wave = wave_id(), lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
   const int w0 = r0 + wave * (16 * RT);
 
-  h8 q[RT][2 * C];
-  float scale[RT];
-  int end[RT];
-#pragma unroll
-  for (int t = 0; t < RT; t++) {
-    const int r = min(w0 + 16 * t + col, packed - 1), i = r / c.group;
-    end[t] = c.causal ? base + i + 1 : length;
-    scale[t] = load_query<D, DT>(c, row0 + i, kvh * c.group + r % c.group, quad, q[t]);
-  }
   const int window = c.window ? c.window : INT32_MAX;  // a row sees tokens end - window .. end - 1
 
   // blocks that some row of the workgroup sees, and the tokens that some, or all, of the wave's rows do
@@ -102,12 +93,14 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(Call c, Pool pool, Rows ro
   const auto refill = [&](int b) {
     from_b = b;
     ids = b + lane < stop ? rows.block(seq, b + lane, pool.blocks) : -1;
+  };
+  const auto refill_scales = [&]() {
     const size_t x = pool.scale(max(ids, 0), kvh);
     const float v = pool.vs[x], none = v - v;
     // a value scale of no number makes the logits none, of the rows that see the block
     kss = ids < 0 ? 0.0f : pool.ks[x] + none;
     vss = ids < 0 || none != 0 ? -1.0f : fmaxf(v, 0x1p-126f);
-    until = b;
+    until = from_b;
   };
   const auto lane_value = [&](float v, int b) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), b - from_b));
@@ -126,13 +119,21 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(Call c, Pool pool, Rows ro
 
   refill(first);
   int block = first < stop ? block_at(first) : -1;
-  if (block >= 0) {
-    fetch(block);
-    put(first);
+  if (block >= 0) fetch(block);
+  h8 q[RT][2 * C];
+  float scale[RT];
+  int end[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const int r = min(w0 + 16 * t + col, packed - 1), i = r / c.group;
+    end[t] = c.causal ? base + i + 1 : length;
+    scale[t] = load_query<D, DT>(c, row0 + i, kvh * c.group + r % c.group, quad, q[t]);
   }
+  refill_scales();
+  if (block >= 0) put(first);
   __syncthreads();
   for (int b = first; b < stop; b++) {
-    if (b - from_b > 62) refill(b);
+    if (b - from_b > 62) refill(b), refill_scales();
     const int next = block_at(b + 1);
     if (next >= 0) fetch(next);
     const int p0 = b * BLOCK;
@@ -239,45 +240,53 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(Call c, Pool pool, Rows ro
     __syncthreads();
   }
 
+  // Out through LDS, a tile of the wave's at a time, so that rows are written whole.
+  constexpr int PITCH = D + 8;
+  uint16_t *const turned = (uint16_t *)held + wave * (16 * PITCH);
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     float sum = l[t];
     sum += lane_xor16(sum);
     sum += lane_xor32(sum);
-    const int r = w0 + 16 * t + col;
-    if (r >= packed) continue;
-    const size_t at = (size_t)(row0 + r / c.group) * c.heads + kvh * c.group + r % c.group;
     const float by = c.splits > 1 ? unit : sum == 0 ? 0.0f : unit / sum;
-    const size_t to = (size_t)split * rows.rows * c.heads + at;
+    const auto place = [&](int i) {  // of row i of the tile in out
+      const int r = w0 + 16 * t + i;
+      return (size_t)(row0 + r / c.group) * c.heads + kvh * c.group + r % c.group;
+    };
+    if (c.splits > 1) {
+      if (w0 + 16 * t + col >= packed) continue;
+      const size_t to = (size_t)split * rows.rows * c.heads + place(col);
+#pragma unroll
+      for (int d = 0; d < V; d++) *(f4 *)(c.part + to * D + 16 * d + 4 * quad) = o[t][d] * by;
+      if (quad == 0) c.ml[to] = float2{m[t], sum};
+      continue;
+    }
 #pragma unroll
     for (int d = 0; d < V; d++) {
-      f4 x = o[t][d];
-#pragma unroll
-      for (int i = 0; i < 4; i++) x[i] *= by;
-      if (c.splits == 1) *(u2 *)((uint16_t *)c.out + at * D + 16 * d + 4 * quad) = u2{narrow2<DT>(x[0], x[1]), narrow2<DT>(x[2], x[3])};
-      else *(f4 *)(c.part + to * D + 16 * d + 4 * quad) = x;
+      const f4 x = o[t][d] * by;
+      *(u2 *)(turned + col * PITCH + 16 * d + 4 * quad) = u2{narrow2<DT>(x[0], x[1]), narrow2<DT>(x[2], x[3])};
     }
-    if (c.splits > 1 && quad == 0) c.ml[to] = float2{m[t], sum};
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+      const int r = (64 * i + lane) / (D / 8), d = (64 * i + lane) % (D / 8) * 8;
+      const u4 x = *(const u4 *)(turned + r * PITCH + d);
+      if (w0 + 16 * t + r < packed) *(u4 *)((uint16_t *)c.out + place(r) * D + d) = x;
+    }
   }
 }
 
-// Row tiles of a wave. Heads of 128: two (535 us for 8192 tokens; three 532, one more block of work in the last
-// workgroup). Heads of 64 one (three sequences of 12000 tokens and 1500 rows of 8 heads over one: 95 us; two 96, with
-// half the workgroups for short calls); heads of 256 one, two spill.
-template <int D>
-constexpr int ROW_TILES = D == 128 ? 2 : 1;
-int tile_rows(int dim) { return 128 * (dim == 128 ? ROW_TILES<128> : ROW_TILES<64>); }
-
-template <int D, int FMT, int DT>
+template <int D, int FMT, int DT, int RT>
 static void launch(const Call &c, const Pool &pool, const Rows &rows, int tiles, uint32_t total, hipStream_t st) {
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_kernel<D, FMT, DT, ROW_TILES<D>>), dim3(total), dim3(512), 2 * 16 * (D / 64) * 1024, st, c, pool,
-                     rows, tiles);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_kernel<D, FMT, DT, RT>), dim3(total), dim3(512), 2 * 16 * (D / 64) * 1024, st, c, pool, rows,
+                     tiles);
 }
-void launch_tile(const Call &c, const Pool &pool, const Rows &rows, int format, int dtype, int tiles, uint32_t total, hipStream_t st) {
-#define ISHZ_TILE_D(F, T)                                               \
-  if (pool.dim == 64) launch<64, F, T>(c, pool, rows, tiles, total, st);     \
-  else if (pool.dim == 128) launch<128, F, T>(c, pool, rows, tiles, total, st); \
-  else launch<256, F, T>(c, pool, rows, tiles, total, st)
+void launch_tile(const Call &c, const Pool &pool, const Rows &rows, int format, int dtype, int row_tiles, int tiles, uint32_t total,
+                 hipStream_t st) {
+#define ISHZ_TILE_D(F, T)                                                                \
+  if (pool.dim == 64) launch<64, F, T, 1>(c, pool, rows, tiles, total, st);               \
+  else if (pool.dim == 256) launch<256, F, T, 1>(c, pool, rows, tiles, total, st);        \
+  else if (row_tiles == 1) launch<128, F, T, 1>(c, pool, rows, tiles, total, st);         \
+  else launch<128, F, T, 2>(c, pool, rows, tiles, total, st)
   if (format == ISHZ_KV_INT8) {
     if (dtype == ISHZ_DT_F16) { ISHZ_TILE_D(ISHZ_KV_INT8, ISHZ_DT_F16); } else { ISHZ_TILE_D(ISHZ_KV_INT8, ISHZ_DT_BF16); }
   } else {

@@ -156,14 +156,13 @@ __global__ __launch_bounds__(256) void append_kernel(Heads k, Heads v, Heads q, 
     for (int m = 0; m < N; m++)  // slots past the last read the last one's token again: whole heads take part in a norm
       raw[m].load(k.x, (size_t)((int64_t)(row_of + min(s0 + (tid + 256 * m) / U, s1 - 1)) * k.row + head * k.head), ca, cb);
     unrolled<N>([&](auto m) __attribute__((always_inline)) {
+      if (256 * m / U >= s1 - s0) return;  // the same for the whole workgroup
       raw[m].widen(x[m]);
-      if (256 * m / U < s1 - s0) {  // the same for the whole workgroup
-        if (k.weight) unit_norm<U>(x[m], w, eps);
-        if (u < t.rot / 16) {
-          float c[8], s[8];
-          unit_angles(t, u, t.positions[row_of + min(s0 + (tid + 256 * m) / U, s1 - 1)], c, s);
-          unit_turn(t.interleaved, c, s, x[m]);
-        }
+      if (k.weight) unit_norm<U>(x[m], w, eps);
+      if (u < t.rot / 16) {
+        float c[8], s[8];
+        unit_angles(t, u, t.positions[row_of + min(s0 + (tid + 256 * m) / U, s1 - 1)], c, s);
+        unit_turn(t.interleaved, c, s, x[m]);
       }
 #pragma unroll
       for (int i = 0; i < 16; i++) larger(x[m][i]);

@@ -275,6 +275,29 @@ def test_append_with_norms_and_rotation(dtype, dim, rot, interleaved):
     model.check(cache, key_error=2.0 ** -18)  # see rope_tolerance: 2^-19 sqrt 2 of the head's largest
 
 
+@pytest.mark.parametrize("dtype", [INT8, E4M3])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 9, 31])
+def test_append_takes_scales_from_normed_keys(dtype, dim, rows):
+    """Keys far larger before their norm than after it, into partly filled blocks whose scales hold the latter: the scales
+    stay. The same keys without a norm make them grow."""
+    batch, blocks = make_batch([20 + rows, 61 + rows], [rows, rows], seed=3)
+    first = random_cache(blocks, 2, dim, dtype, seed=8)
+    k = normal(5, 2 * rows, 2, dim, dtype=BF16) * 50
+    w = torch.full((dim,), 0.5)
+    for weight in (w, None):
+        cache = gpu(first)
+        model = Model(cache)
+        x = rope_reference(k, None, [], weight, 1e-6, False)
+        attention.append(k.to(DEV), k.to(DEV), cache, batch, k_weight=None if weight is None else weight.to(DEV))
+        for s in range(2):
+            for which, new in enumerate((x, k)):
+                model.append(which, new[s * rows:s * rows + rows], batch.table[s].tolist(), (20, 61)[s])
+        model.check(cache, key_error=2.0 ** -18)
+        grown = cache.k_scale[batch.table[0, 0].item()].cpu() > first.k_scale[batch.table[0, 0].item()]
+        assert bool(grown.any()) == (weight is None)
+
+
 def test_append_again_changes_nothing():
     batch, blocks = make_batch([70, 3], [7, 2])
     cache = gpu(random_cache(blocks, 2, 128, INT8, seed=9))

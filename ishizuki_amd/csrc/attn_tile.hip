@@ -34,6 +34,15 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(Call c, Pool pool, Rows ro
   const int wave = wave_id(), lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
   const int w0 = r0 + wave * (16 * RT);
 
+  h8 q[RT][2 * C];
+  float scale[RT];
+  int end[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const int r = min(w0 + 16 * t + col, packed - 1), i = r / c.group;
+    end[t] = c.causal ? base + i + 1 : length;
+    scale[t] = load_query<D, DT>(c, row0 + i, kvh * c.group + r % c.group, quad, q[t]);
+  }
   const int window = c.window ? c.window : INT32_MAX;  // a row sees tokens end - window .. end - 1
 
   // blocks that some row of the workgroup sees, and the tokens that some, or all, of the wave's rows do
@@ -120,15 +129,6 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(Call c, Pool pool, Rows ro
   refill(first);
   int block = first < stop ? block_at(first) : -1;
   if (block >= 0) fetch(block);
-  h8 q[RT][2 * C];
-  float scale[RT];
-  int end[RT];
-#pragma unroll
-  for (int t = 0; t < RT; t++) {
-    const int r = min(w0 + 16 * t + col, packed - 1), i = r / c.group;
-    end[t] = c.causal ? base + i + 1 : length;
-    scale[t] = load_query<D, DT>(c, row0 + i, kvh * c.group + r % c.group, quad, q[t]);
-  }
   refill_scales();
   if (block >= 0) put(first);
   __syncthreads();

@@ -8,17 +8,17 @@ namespace attn {
 // worked on, the next one's codes are on their way in registers. As in stream_kernel S^T = K Q^T leaves a lane the
 // weights of 16 consecutive tokens of a row, which are the operands of O^T += V^T P^T as they are.
 //
-// Sums stay in the units of a reference that is only moved when a logit passes it by 2^8 (weights stay below fp16's
-// largest), and of a value scale `unit` that blocks' scales are 1..255 of: log2 of that ratio is added to the block's
-// logits, so that nothing but the matrix units touches the sums. A block outside 1..255 moves the unit, which stays above
-// 2^-80 of the largest scale (the sums' 2^45 then stay finite).
+// A row's sums stay in the units of a reference that is only moved when a logit passes it by 2^8 (weights stay below
+// fp16's largest), and of a value scale `unit` that the scales of the blocks it sees are 1..255 of: log2 of that ratio is
+// added to the block's logits, so that nothing but the matrix units touches the sums. A block outside 1..255 moves the
+// unit, which stays above 2^-72 of the largest scale the row has seen (the sums' 2^45 then stay finite).
 //
 // Power bounds it: these products alone, from registers, run at 1970 TFLOP/s on such values (1700 as 32x32x16) where the
 // clock would allow 2500, and a library product of 8192 x 8192 x 8192 at 1250 to 1500; 8192 tokens of 32 heads over 8 of
 // 128, causal, take 535 us (1030 TFLOP/s). That time is within 4 % for 16 to 48 rows a wave, products of either
 // shape, vector operations dealt between the products or not, and codes unpacked by a pass before.
 template <int D, int FMT, int DT, int RT>
-__global__ __launch_bounds__(512, 2) void tile_kernel(Call c, Pool pool, Rows rows, int tiles) {
+__global__ __launch_bounds__(512, RT * D <= 128 ? 4 : 2) void tile_kernel(Call c, Pool pool, Rows rows, int tiles) {
   constexpr int C = D / 64, V = D / 16;
   extern __shared__ h8 held[];  // [2][16 C operands][64]
   int id = blockIdx.x;
@@ -87,18 +87,17 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(Call c, Pool pool, Rows ro
   };
 
   f4 o[RT][V];
-  float m[RT], l[RT];
-  float unit = 0x1p-100f, largest = 0;
+  float m[RT], l[RT], unit[RT], inv[RT], largest[RT];
 #pragma unroll
   for (int t = 0; t < RT; t++) {
-    m[t] = -3e38f, l[t] = 0;
+    m[t] = -3e38f, l[t] = 0, unit[t] = 0x1p-100f, inv[t] = 0x1p100f, largest[t] = 0;
 #pragma unroll
     for (int d = 0; d < V; d++) o[t][d] = f4{0, 0, 0, 0};
   }
-  // The numbers of 64 blocks from `from_b` on and what their scales come to, a lane each: read one by one where they are
-  // needed, they would be two dependent loads' latency in every step. The unit stays as it is up to `until`.
-  int ids = -1, from_b = first, until = first;
-  float kss = 0, vss = 0, logs = 0, backs = 1;
+  // The numbers and scales of 64 blocks from `from_b` on, a lane each: read one by one where they are needed, they would be
+  // two dependent loads' latency in every step.
+  int ids = -1, from_b = first;
+  float kss = 0, vss = 0;
   const auto refill = [&](int b) {
     from_b = b;
     ids = b + lane < stop ? rows.block(seq, b + lane, pool.blocks) : -1;
@@ -109,136 +108,143 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(Call c, Pool pool, Rows ro
     // a value scale of no number makes the logits none, of the rows that see the block
     kss = ids < 0 ? 0.0f : pool.ks[x] + none;
     vss = ids < 0 || none != 0 ? -1.0f : fmaxf(v, 0x1p-126f);
-    until = from_b;
   };
   const auto lane_value = [&](float v, int b) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), b - from_b));
   };
   const auto block_at = [&](int b) { return __builtin_amdgcn_readlane(ids, b - from_b); };
-  // The unit of blocks b .. until - 1.
-  const auto set_unit = [&](int b) {
-    const float v = lane_value(vss, b);
-    if (v > 0) largest = fmaxf(largest, v), unit = fmaxf(fmaxf(v * 0x1p-4f, 0x1p-80f * largest), 0x1p-100f);
-    const float ratio = vss < 0 ? 1.0f : fmaxf(vss / unit, 0x1p-64f);
-    logs = __builtin_amdgcn_logf(ratio), backs = 1.0f / ratio;
-    const bool out = ratio > 255.0f || (ratio < 1.0f && vss > 0x1p-76f * largest && vss > 0x1p-100f);
-    const uint64_t off = __ballot(out) >> (b - from_b) >> 1;
-    until = off ? b + 1 + __builtin_ctzll(off) : from_b + 64;
-  };
-
   refill(first);
   int block = first < stop ? block_at(first) : -1;
   if (block >= 0) fetch(block);
   refill_scales();
   if (block >= 0) put(first);
   __syncthreads();
-  for (int b = first; b < stop; b++) {
-    if (b - from_b > 62) refill(b), refill_scales();
-    const int next = block_at(b + 1);
-    if (next >= 0) fetch(next);
-    const int p0 = b * BLOCK;
-    if (block >= 0 && p0 < some1 && p0 + BLOCK > some0) {
-      const float was = unit;
-      if (b >= until) set_unit(b);
-      const float ks = lane_value(kss, b), shift = lane_value(logs, b), back = lane_value(backs, b);
-      const h8 *const at = held + ((b - first) & 1) * (16 * C * 64) + lane;
-      h8 a = at[0], a2 = at[64];
-      f4 s[RT][4];
+  // Blocks b .. stop - 1; `apart`: what each brings is added in 32 bits. Without, a wave returns at the first block that needs
+  // that, with its work on it still to be done.
+  const auto pass = [&](auto apart, int b) {
+    for (; b < stop; b++) {
+      if (b - from_b > 62) refill(b), refill_scales();
+      const int next = block_at(b + 1);
+      if (next >= 0) fetch(next);
+      const int p0 = b * BLOCK;
+      if (block >= 0 && p0 < some1 && p0 + BLOCK > some0) {
+        const float ks = lane_value(kss, b), vb = lane_value(vss, b);
+        const h8 *const at = held + ((b - first) & 1) * (16 * C * 64) + lane;
+        h8 a = at[0], a2 = at[64];
+        f4 s[RT][4];
 #pragma unroll
-      for (int x = 0; x < 4 * C; x++) {
-        const h8 y = at[(2 * x + 2) * 64], y2 = at[(2 * x + 3) * 64];
-        __builtin_amdgcn_sched_barrier(0);
-        const int t = x / C;
+        for (int x = 0; x < 4 * C; x++) {
+          const h8 y = at[(2 * x + 2) * 64], y2 = at[(2 * x + 3) * 64];
+          __builtin_amdgcn_sched_barrier(0);
+          const int t = x / C;
 #pragma unroll
-        for (int r = 0; r < RT; r++) s[r][t] = mfma32(a, q[r][2 * (x % C)], x % C ? s[r][t] : f4{0, 0, 0, 0});
+          for (int r = 0; r < RT; r++) s[r][t] = mfma32(a, q[r][2 * (x % C)], x % C ? s[r][t] : f4{0, 0, 0, 0});
 #pragma unroll
-        for (int r = 0; r < RT; r++) s[r][t] = mfma32(a2, q[r][2 * (x % C) + 1], s[r][t]);
-        a = y, a2 = y2;
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      float f[RT];
+          for (int r = 0; r < RT; r++) s[r][t] = mfma32(a2, q[r][2 * (x % C) + 1], s[r][t]);
+          a = y, a2 = y2;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        float f[RT], ratio[RT];
 #pragma unroll
-      for (int r = 0; r < RT; r++) f[r] = scale[r] * ks;
-      if (p0 < whole0 || p0 + BLOCK > whole1) {
+        for (int r = 0; r < RT; r++) f[r] = scale[r] * ks, ratio[r] = vb < 0 ? 1.0f : vb * inv[r];
+        if (p0 < whole0 || p0 + BLOCK > whole1) {
+#pragma unroll
+          for (int r = 0; r < RT; r++) {
+            const int before = end[r] - 1 - (p0 + 16 * quad);  // tokens between the lane's first and the row's last
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                s[r][t][i] = before >= 4 * t + i && before - (4 * t + i) < window ? s[r][t][i] * f[r] : -__builtin_inff();
+            f[r] = 1;
+            if (end[r] <= p0 || end[r] - p0 >= (int64_t)window + BLOCK) ratio[r] = 1;  // sees none of the block
+          }
+        }
+        float top[RT];
+        bool move = false;
 #pragma unroll
         for (int r = 0; r < RT; r++) {
-          const int before = end[r] - 1 - (p0 + 16 * quad);  // tokens between the lane's first and the row's last
+          float x = s[r][0][0];
 #pragma unroll
           for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              s[r][t][i] = before >= 4 * t + i && before - (4 * t + i) < window ? s[r][t][i] * f[r] : -__builtin_inff();
-          f[r] = 1;
+            for (int i = 0; i < 4; i++) x = fmaxf(x, s[r][t][i]);
+          top[r] = x * f[r];
+          move |= top[r] > m[r] + 8.0f || ratio[r] > 255.0f || (ratio[r] < 1.0f && vb > 0x1p-120f);  // all zeros: moves nothing
         }
-      }
-      float top[RT];
-      bool move = false;
+        bool below = false;
+        if (__any(move)) {
 #pragma unroll
-      for (int r = 0; r < RT; r++) {
-        float x = s[r][0][0];
+          for (int r = 0; r < RT; r++) {
+            float x = fmaxf(top[r], m[r]);
+            x = fmaxf(x, lane_xor16(x));
+            x = fmaxf(x, lane_xor32(x));
+            float alpha = __builtin_amdgcn_exp2f(m[r] - x);
+            m[r] = x;
+            l[r] *= alpha;
+            if (ratio[r] > 255.0f || (ratio[r] < 1.0f && vb > 0x1p-120f)) {
+              largest[r] = fmaxf(fmaxf(largest[r], 256.0f * unit[r]), vb);
+              const float to = fmaxf(fmaxf(vb * 0x1p-4f, 0x1p-72f * largest[r]), 0x1p-100f);
+              alpha *= unit[r] / to;
+              unit[r] = to, inv[r] = 1.0f / to, ratio[r] = vb * inv[r];
+              below |= ratio[r] < 1.0f;
+            }
 #pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) x = fmaxf(x, s[r][t][i]);
-        top[r] = x * f[r];
-        move |= top[r] > m[r] + 8.0f;
-      }
-      if (unit != was || __any(move)) {
-        const float units = was / unit;
-#pragma unroll
-        for (int r = 0; r < RT; r++) {
-          float x = fmaxf(top[r], m[r]);
-          x = fmaxf(x, lane_xor16(x));
-          x = fmaxf(x, lane_xor32(x));
-          const float alpha = __builtin_amdgcn_exp2f(m[r] - x);
-          m[r] = x;
-          l[r] *= alpha;
-#pragma unroll
-          for (int d = 0; d < V; d++) {  // one after another: the compiler holds all of them twice otherwise
-            f4 y = o[r][d] * (alpha * units);
-            asm volatile("" : "+v"(y));
-            o[r][d] = y;
-            __builtin_amdgcn_sched_barrier(0);
+            for (int d = 0; d < V; d++) {  // one after another: the compiler holds all of them twice otherwise
+              f4 y = o[r][d] * alpha;
+              asm volatile("" : "+v"(y));
+              o[r][d] = y;
+              __builtin_amdgcn_sched_barrier(0);
+            }
           }
         }
-      }
-      h8 p[RT][2];
+        if (!apart && __any(below)) return b;
+        h8 p[RT][2];
 #pragma unroll
-      for (int r = 0; r < RT; r++) {
-        const float ref = shift - m[r];
-        float sum = 0;
+        for (int r = 0; r < RT; r++) {
+          const float part_of = apart ? 1.0f : fmaxf(ratio[r], 0x1p-64f), ref = __builtin_amdgcn_logf(part_of) - m[r];
+          float sum = 0;
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-          typedef float f2 __attribute__((ext_vector_type(2)));
-          const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][0], f[r], ref));
-          const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][1], f[r], ref));
-          const float w2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][2], f[r], ref));
-          const float w3 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][3], f[r], ref));
-          sum += (w0 + w1) + (w2 + w3);
-          // Weights are rounded to fp16 for the matrix units: 2^-12 of each, the sums stay in 32 bits.
-          const h2 lo = __builtin_convertvector((f2{w0, w1}), h2), hi = __builtin_convertvector((f2{w2, w3}), h2);
-          p[r][t / 2][4 * (t % 2)] = lo.x, p[r][t / 2][4 * (t % 2) + 1] = lo.y;
-          p[r][t / 2][4 * (t % 2) + 2] = hi.x, p[r][t / 2][4 * (t % 2) + 3] = hi.y;
+          for (int t = 0; t < 4; t++) {
+            typedef float f2 __attribute__((ext_vector_type(2)));
+            const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][0], f[r], ref));
+            const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][1], f[r], ref));
+            const float w2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][2], f[r], ref));
+            const float w3 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][3], f[r], ref));
+            sum += (w0 + w1) + (w2 + w3);
+            // Weights are rounded to fp16 for the matrix units: 2^-12 of each, the sums stay in 32 bits.
+            const h2 lo = __builtin_convertvector((f2{w0, w1}), h2), hi = __builtin_convertvector((f2{w2, w3}), h2);
+            p[r][t / 2][4 * (t % 2)] = lo.x, p[r][t / 2][4 * (t % 2) + 1] = lo.y;
+            p[r][t / 2][4 * (t % 2) + 2] = hi.x, p[r][t / 2][4 * (t % 2) + 3] = hi.y;
+          }
+          l[r] += sum * __builtin_amdgcn_rcpf(part_of);
         }
-        l[r] += sum * back;
+#pragma unroll
+        for (int d = 0; d < V; d++) {
+          h8 y = a, y2 = a2;
+          if (d + 1 < V) y = at[(8 * C + 2 * d + 2) * 64], y2 = at[(8 * C + 2 * d + 3) * 64];
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (apart) {
+#pragma unroll
+            for (int r = 0; r < RT; r++) o[r][d] += mfma32(a2, p[r][1], mfma32(a, p[r][0], f4{0, 0, 0, 0})) * ratio[r];
+          } else {
+#pragma unroll
+            for (int r = 0; r < RT; r++) o[r][d] = mfma32(a, p[r][0], o[r][d]);
+#pragma unroll
+            for (int r = 0; r < RT; r++) o[r][d] = mfma32(a2, p[r][1], o[r][d]);
+          }
+          a = y, a2 = y2;
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
-#pragma unroll
-      for (int d = 0; d < V; d++) {
-        h8 y = a, y2 = a2;
-        if (d + 1 < V) y = at[(8 * C + 2 * d + 2) * 64], y2 = at[(8 * C + 2 * d + 3) * 64];
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int r = 0; r < RT; r++) o[r][d] = mfma32(a, p[r][0], o[r][d]);
-#pragma unroll
-        for (int r = 0; r < RT; r++) o[r][d] = mfma32(a2, p[r][1], o[r][d]);
-        a = y, a2 = y2;
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      if (next >= 0) put(b + 1);
+      block = next;
+      __syncthreads();
     }
-    if (next >= 0) put(b + 1);
-    block = next;
-    __syncthreads();
-  }
+    return b;
+  };
+  const int rest = pass(std::false_type{}, first);
+  if (rest < stop) pass(std::true_type{}, rest);
 
   // Out through LDS, a tile of the wave's at a time, so that rows are written whole.
   constexpr int PITCH = D + 8;
@@ -248,7 +254,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(Call c, Pool pool, Rows ro
     float sum = l[t];
     sum += lane_xor16(sum);
     sum += lane_xor32(sum);
-    const float by = c.splits > 1 ? unit : sum == 0 ? 0.0f : unit / sum;
+    const float by = c.splits > 1 ? unit[t] : sum == 0 ? 0.0f : unit[t] / sum;
     const auto place = [&](int i) {  // of row i of the tile in out
       const int r = w0 + 16 * t + i;
       return (size_t)(row0 + r / c.group) * c.heads + kvh * c.group + r % c.group;

@@ -452,6 +452,69 @@ def test_attend_ignores_what_it_does_not_see(dtype, rows):
     assert not got[first].isnan().any()
 
 
+WIDE = [  # lengths, rows, causal, window: what the kernels for more rows, longer caches and several splits get to see
+    ([700], [33], True, 0), ([4500, 300], [20, 17], True, 0), ([9000], [70], True, 0), ([8300, 9000], [40, 66], True, 500),
+    ([1030], [1030], True, 0), ([1500], [130], False, 0), ([5000], [9], True, 0), ([400, 1000], [1, 1], True, 0),
+]
+
+
+@pytest.mark.parametrize("lengths,rows,causal,window", WIDE)
+@pytest.mark.parametrize("heads,group,dim,dtype,x", [(1, 4, 128, INT8, BF16), (2, 1, 64, E4M3, F16), (1, 2, 256, INT8, F16)])
+def test_attend_longer(lengths, rows, causal, window, heads, group, dim, dtype, x):
+    print(f"attend {lengths} {rows} {causal} {window} {heads} x {group} x {dim} {dtype} {x}", flush=True)
+    batch, blocks = make_batch(lengths, rows, seed=1)
+    cache = random_cache(blocks, heads, dim, dtype, seed=sum(lengths))
+    q = normal(3, sum(rows), heads * group, dim, dtype=x)
+    got = attention.attend(q.to(DEV), gpu(cache), batch, causal=causal, window=window)
+    attention_close(got, q, attention_reference(q, cache, batch, dim ** -0.5, causal, window))
+
+
+def test_attend_many_blocks_a_workgroup():
+    """Caches of more blocks than a wave holds the numbers of, not split, with holes."""
+    n, length = 64, 4500
+    batch, blocks = make_batch([length] * n, [18] * n, seed=1)
+    batch.table[:, 3], batch.table[5, 61:64], batch.table[:, 65] = -1, blocks, -7
+    cache = random_cache(blocks, 4, 64, INT8, seed=7)
+    q = normal(3, 18 * n, 4, 64, dtype=F16)
+    got = attention.attend(q.to(DEV), gpu(cache), batch)
+    for s in (0, 5, 63):
+        one = attention.Batch(batch.table[s:s + 1], i32(length), i32(0, 18), 18, length)
+        rows = slice(18 * s, 18 * s + 18)
+        attention_close(got[rows], q[rows], attention_reference(q[rows], cache, one, 0.125, True, 0))
+
+
+def visible(cache, batch, rows, length, window, group):
+    """Sums of |v| over the tokens that each row sees, [rows, q heads, dim] in 64 bits."""
+    _, v = values(cache, batch, 0, length)
+    total = torch.cat((torch.zeros_like(v[:1]), v.abs().nan_to_num().cumsum(0)))
+    end = length - rows + torch.arange(rows) + 1
+    begin = (end - window).clamp(min=0) if window else torch.zeros_like(end)
+    return (total[end] - total[begin]).repeat_interleave(group, 1)
+
+
+@pytest.mark.parametrize("dtype", [INT8, E4M3])
+@pytest.mark.parametrize("rows,window", [(3, 0), (300, 0), (300, 20), (640, 64), (40, 7)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attend_value_scales_far_apart(dtype, rows, window, dim):
+    """Blocks whose values differ by up to 2^100, and one that is all zeros with scales of 0: a row that sees none of the
+    large ones is as exact as if they were not there. Weights below fp16's normals are off by 2^-25 of the largest each."""
+    length = 640
+    batch, blocks = make_batch([length], [rows], seed=2)
+    cache = random_cache(blocks, 1, dim, dtype, seed=6)
+    for j, e in enumerate([0, -30, 12, -45, 3, -3, 40, -60, 0, 9]):
+        cache.v_scale[batch.table[0, j].item()] *= 2.0 ** e
+    zero = batch.table[0, 4].item()
+    cache.v_scale[zero], cache.k_scale[zero] = 0, 0
+    cache.v.view(INT8)[zero] = 0
+    q = normal(3, rows, 2, dim, dtype=BF16)
+    out, bound, shift = attention_reference(q, cache, batch, dim ** -0.5, True, window)
+    got = attention.attend(q.to(DEV), gpu(cache), batch, window=window).cpu().double()
+    tol = u(BF16) * out.abs() + (2.0 ** -11 + 2.0 ** -19 + 2 * (dim + 8) * u(F32) * shift) * bound
+    tol = tol + 2.0 ** -25 * visible(cache, batch, rows, length, window, 2) + 2.0 ** -126
+    d = (got - out).abs()
+    assert torch.all(d <= tol), float((d / tol).max())
+
+
 def test_strides_streams_and_rows_of_no_sequence():
     batch, blocks = make_batch([100, 40], [2, 3], seed=4)
     cache = random_cache(blocks, 2, 128, INT8, seed=6)

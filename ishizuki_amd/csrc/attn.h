@@ -241,8 +241,8 @@ DEV float load_query(const Call &c, int64_t row, int head, int quad, h8 *q) {
   return scale;
 }
 
-// tile_kernel (attn_tile.hip) with 128 row_tiles packed rows to a workgroup (two only of heads of 128), `tiles` workgroups a
-// sequence, head and split.
+// tile_kernel (attn_tile.hip) with 128 row_tiles packed rows to a workgroup (of heads of 256 128), `tiles` workgroups a sequence,
+// head and split.
 void launch_tile(const Call &c, const Pool &pool, const Rows &rows, int format, int dtype, int row_tiles, int tiles, uint32_t total,
                  hipStream_t st);
 

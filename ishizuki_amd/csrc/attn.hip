@@ -28,6 +28,15 @@ __global__ __launch_bounds__(64 * W) void stream_kernel(Call c, Pool pool, Rows 
   if (r0 >= packed) return;
   const int wave = wave_id(), lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
 
+  // blocks that some row sees; those that every row sees whole need no mask
+  const int i0 = r0 / c.group, i1 = (min(r0 + 16 * RT, packed) - 1) / c.group;
+  const int last = c.causal ? base + i1 + 1 : length, from = c.window ? max(base + i0 + 1 - c.window, 0) : 0;
+  const int whole0 = c.window ? max(base + i1 + 1 - c.window, 0) : 0, whole1 = c.causal ? base + i0 + 1 : length;
+  const int b0 = from / BLOCK, b1 = max((last + BLOCK - 1) / BLOCK, b0);
+  const int each = (b1 - b0 + c.splits - 1) / c.splits;
+  const int first = b0 + split * each, stop = min(first + each, b1);
+
+  int next = first + wave < stop ? rows.block(seq, first + wave, pool.blocks) : -1;
   // the rows, and the tokens that each sees: begin[] .. end[] - 1
   h8 q[RT][2 * C];
   float scale[RT];
@@ -40,14 +49,6 @@ __global__ __launch_bounds__(64 * W) void stream_kernel(Call c, Pool pool, Rows 
     scale[t] = load_query<D, DT>(c, row0 + i, kvh * c.group + r % c.group, quad, q[t]);
   }
 
-  // blocks that some row sees; those that every row sees whole need no mask
-  const int i0 = r0 / c.group, i1 = (min(r0 + 16 * RT, packed) - 1) / c.group;
-  const int last = c.causal ? base + i1 + 1 : length, from = c.window ? max(base + i0 + 1 - c.window, 0) : 0;
-  const int whole0 = c.window ? max(base + i1 + 1 - c.window, 0) : 0, whole1 = c.causal ? base + i0 + 1 : length;
-  const int b0 = from / BLOCK, b1 = max((last + BLOCK - 1) / BLOCK, b0);
-  const int each = (b1 - b0 + c.splits - 1) / c.splits;
-  const int first = b0 + split * each, stop = min(first + each, b1);
-
   f4 o[RT][V];
   float m[RT], l[RT];
 #pragma unroll
@@ -56,7 +57,6 @@ __global__ __launch_bounds__(64 * W) void stream_kernel(Call c, Pool pool, Rows 
 #pragma unroll
     for (int d = 0; d < V; d++) o[t][d] = f4{0, 0, 0, 0};
   }
-  int next = first + wave < stop ? rows.block(seq, first + wave, pool.blocks) : -1;
   for (int b = first + wave; b < stop; b += W) {
     const int block = __builtin_amdgcn_readfirstlane(next);
     next = b + W < stop ? rows.block(seq, b + W, pool.blocks) : -1;
@@ -262,9 +262,11 @@ static Plan plan(int q_heads, int heads, int dim, int sequences, int max_rows, i
       splits = std::min(std::max((1024 + pairs - 1) / pairs, blocks / 32), (blocks + 3) / 4);
     }
   } else {
-    // 256 rows a workgroup halve the decoding: for many (4096 tokens of 32 heads over 8: 150 us, 128 rows 185), or few rows
-    // over a long cache (512 over 16384: 148 and 158). Otherwise 128 rows end more evenly (2048 tokens: 59 us, 72).
-    const bool wide = dim == 128 && packed > 128 && (pairs * tiles(256) >= 512 || (blocks >= 128 && max_length >= 4 * (int64_t)max_rows));
+    // 256 rows a workgroup halve the decoding: for many of heads of 128 (4096 tokens of 32 heads over 8: 150 us, 128 rows
+    // 185; of 64 114 and 118), or few rows over a long cache (512 over 16384: 148 and 158; of 64 108 and 134). Otherwise 128
+    // rows end more evenly (2048 tokens: 59 us, 72; of 64 42 and 53).
+    const bool wide = packed > 128 && ((dim == 128 && pairs * tiles(256) >= 512) ||
+                                       (dim < 256 && blocks >= 128 && max_length >= 4 * (int64_t)max_rows));
     p.row_tiles = wide ? 2 : 1;
     p.tiles = (int)tiles(128 * p.row_tiles);
     // A workgroup a CU, and at least six blocks each (128 rows over 4096 tokens: one split 83 us, eight 24; 512 tokens among

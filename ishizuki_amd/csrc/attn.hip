@@ -242,27 +242,29 @@ struct Plan {
   bool stream;  // stream_kernel, or tile_kernel
   int row_tiles, tiles, splits, waves;
 };
-static Plan plan(int q_heads, int heads, int dim, int sequences, int max_rows, int max_length) {
+static Plan plan(int q_heads, int heads, int dim, int sequences, int max_rows, int max_length, int window) {
   Plan p;
   const int64_t packed = (int64_t)max_rows * (q_heads / heads), blocks = ((int64_t)max_length + BLOCK - 1) / BLOCK;
   const int64_t pairs = std::max<int64_t>((int64_t)sequences * heads, 1);
+  // Blocks that a workgroup's rows see: a window of 1000 over 32768 tokens is one row's 17 (9.0 us, 11.2 divided as 512).
+  const int64_t span = window ? std::min(blocks, ((int64_t)window + std::min(max_rows, 256) + 62) / BLOCK + 1) : blocks;
   const auto tiles = [&](int per) { return (packed + per - 1) / per; };
   // Sixteen packed rows or fewer stream; of heads of 256, whose codes take most of the registers, only while a wave has
   // but a few blocks (64 blocks of 2 heads: 11.9 us, tiles 13.3; 256 of 32: 82 and 61). Up to 32 rows do of heads of 128
   // (four sequences of 8191 tokens, 8 heads: 23.8 us, tiles 31.8; of 64 21.3 and 18.5, of 256 38 and 24.5).
-  p.stream = packed <= 16 ? dim < 256 || pairs * blocks < 1024 : packed <= 32 && dim == 128;
+  p.stream = packed <= 16 ? dim < 256 || pairs * span < 1024 : packed <= 32 && dim == 128;
   p.waves = 4;
   int64_t splits;
   if (p.stream) {
     p.row_tiles = packed <= 16 ? 1 : 2;
     p.tiles = (int)tiles(16 * p.row_tiles);
-    if (p.row_tiles == 1 && dim < 256 && blocks > 4 && blocks <= 16) {
+    if (p.row_tiles == 1 && dim < 256 && span > 4 && span <= 16) {
       p.waves = 8;  // two blocks a wave and one launch (13 blocks: 9.6 us; four waves, four splits and their join: 10.1)
       splits = 1;
     } else {
       // Four workgroups a CU, and at most 32 blocks a wave's share of four, so that long sequences beside short ones end
       // sooner (16 sequences of 12000 to 32768 tokens, 8 heads: 138 us, 141 without; 60000 of one: 32.5).
-      splits = std::min(std::max((1024 + pairs - 1) / pairs, blocks / 32), (blocks + 3) / 4);
+      splits = std::min(std::max((1024 + pairs - 1) / pairs, span / 32), (span + 3) / 4);
     }
   } else {
     // 256 rows a workgroup halve the decoding: for many of heads of 128 (4096 tokens of 32 heads over 8: 150 us, 128 rows
@@ -272,11 +274,18 @@ static Plan plan(int q_heads, int heads, int dim, int sequences, int max_rows, i
                                        (dim < 256 && blocks >= 128 && max_length >= 4 * (int64_t)max_rows));
     p.row_tiles = wide ? 2 : 1;
     p.tiles = (int)tiles(128 * p.row_tiles);
-    // A workgroup a CU, and at least six blocks each (128 rows over 4096 tokens: one split 83 us, eight 24; 512 tokens among
-    // themselves: one 17, two 23).
-    splits = std::min(256 / std::max<int64_t>(pairs * p.tiles, 1), blocks / 6);
+    // A workgroup a CU, two where a sequence's rows are one tile and the parts to join few (4 x 8 tokens over 8191 of 32
+    // heads over 8 of 64: 18.5 us, 20.8 with one; 4 x 32 of 128 in a window of 4096: 26.8, two 31.5), and three blocks each
+    // (16 tokens over 1500: 12.2 us, six 14.9). Where rows see nine blocks or fewer on average the join costs more than
+    // that gives (16 tokens over 700: 12.9, unsplit 16.1; over 512 in two splits no gain; 700 among themselves 24 and 20).
+    const int64_t mean = std::min(span, (max_length - max_rows / 2 + BLOCK - 1) / (int64_t)BLOCK);
+    splits = 256 / std::max<int64_t>(pairs * p.tiles, 1);
+    if (splits > 1 && splits <= 8 && dim < 256 && packed * dim <= 8192) splits *= 2;
+    splits = mean < 9 ? 1 : std::min(splits, span / 3);
   }
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, 64));
+  // the workspace's size knows no window
+  if (window) p.splits = std::min(p.splits, plan(q_heads, heads, dim, sequences, max_rows, max_length, 0).splits);
   return p;
 }
 }  // namespace attn
@@ -286,7 +295,7 @@ using namespace attn;
 extern "C" size_t ishz_kv_attend_workspace_size(int rows, int q_heads, int heads, int dim, int sequences, int max_rows,
                                                 int max_length) {
   if (rows < 1 || heads < 1 || q_heads < heads || sequences < 1 || max_rows < 1 || max_length < 1) return 0;
-  const Plan p = plan(q_heads, heads, dim, sequences, std::min(max_rows, rows), max_length);
+  const Plan p = plan(q_heads, heads, dim, sequences, std::min(max_rows, rows), max_length, 0);
   return p.splits == 1 ? 0 : (size_t)p.splits * rows * q_heads * (dim + 2) * 4;
 }
 
@@ -308,7 +317,7 @@ extern "C" int ishz_kv_attend(const void *q, int64_t q_row, int64_t q_head, int 
   max_rows = std::min(max_rows, rows);
   const int group = q_heads / heads;
   if ((int64_t)max_rows * group > INT32_MAX - 64) return ishz::decline("more rows than a launch holds");
-  const Plan p = plan(q_heads, heads, dim, sequences, max_rows, max_length);
+  const Plan p = plan(q_heads, heads, dim, sequences, max_rows, max_length, window);
   const size_t need = p.splits == 1 ? 0 : (size_t)p.splits * rows * q_heads * (dim + 2) * 4;
   if (workspace_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 15)))) return ishz::einval("workspace too small");
   const int64_t total = (int64_t)sequences * heads * p.tiles * p.splits, joins = ((int64_t)rows * q_heads + 3) / 4;

@@ -470,6 +470,18 @@ def test_attend_longer(lengths, rows, causal, window, heads, group, dim, dtype, 
     attention_close(got, q, attention_reference(q, cache, batch, dim ** -0.5, causal, window))
 
 
+@pytest.mark.parametrize("lengths,rows,window", [([9000, 70], [1, 1], 1000), ([5000], [1], 64), ([20000], [1], 257),
+                                                 ([12000, 3], [8, 3], 700), ([6000, 9000], [40, 8], 1500)])
+@pytest.mark.parametrize("heads,group,dim,dtype,x", [(2, 4, 128, INT8, BF16), (2, 3, 64, E4M3, F16), (2, 2, 256, E4M3, BF16)])
+def test_attend_window_of_a_long_cache(lengths, rows, window, heads, group, dim, dtype, x):
+    print(f"attend {lengths} {rows} {window} {heads} x {group} x {dim} {dtype} {x}", flush=True)
+    batch, blocks = make_batch(lengths, rows, seed=1)
+    cache = random_cache(blocks, heads, dim, dtype, seed=sum(lengths))
+    q = normal(3, sum(rows), heads * group, dim, dtype=x)
+    got = attention.attend(q.to(DEV), gpu(cache), batch, window=window)
+    attention_close(got, q, attention_reference(q, cache, batch, dim ** -0.5, True, window))
+
+
 def test_attend_many_blocks_a_workgroup():
     """Caches of more blocks than a wave holds the numbers of, not split, with holes."""
     n, length = 64, 4500

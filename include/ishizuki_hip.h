@@ -274,7 +274,8 @@ int ishz_moe_swiglu(uint32_t type, const void *x, int x_dtype, int T, int H, con
  * of its cache. All three are device memory, read by the kernels, so that a captured call follows them as
  * they change. A sequence may have no rows, or no tokens. An entry of the table outside the pool holds no
  * tokens: what would be written there is dropped, attention leaves it out and reading gives zeros (so blocks
- * behind a window may be freed). Tokens past `width` blocks are none, nor are positions below 0. */
+ * behind a window may be freed). Tokens past `width` blocks are none, nor are positions below 0: a row there is
+ * dropped, and the other rows' positions stay what lengths[s] makes them. */
 enum { ISHZ_KV_BLOCK = 64 };
 enum { ISHZ_KV_INT8 = 0, ISHZ_KV_E4M3 = 1 };
 
@@ -305,8 +306,8 @@ int ishz_kv_append(const void *k, int64_t k_row, int64_t k_head, const void *v, 
                    int interleaved, float factor, const float *q_weight, const float *k_weight, float eps,
                    void *q_out, ishz_stream_t stream);
 
-/* The last `tail` tokens of each sequence: k_out and v_out [sequences][tail][heads][dim] in dtype, zeros
-   where a sequence has fewer. */
+/* The last `tail` tokens of each sequence, those before lengths[s]: k_out and v_out [sequences][tail][heads][dim]
+   in dtype, zeros where a sequence has fewer or its table ends before. */
 int ishz_kv_read(const void *k_codes, const void *v_codes, const float *k_scale, const float *v_scale, int format,
                  int blocks, int heads, int dim, const int32_t *table, int width, const int32_t *lengths,
                  int sequences, int tail, int dtype, void *k_out, void *v_out, ishz_stream_t stream);

@@ -141,8 +141,8 @@ def norm_rope(q, k, positions=None, turns=None, q_weight=None, k_weight=None, ep
 
 def append(k, v, cache, batch, q=None, positions=None, turns=None, q_weight=None, k_weight=None, eps=1e-6,
            interleaved=False, factor=1.0):
-    """Writes k and v [rows, heads, dim] behind what the batch's sequences hold, k normed and turned first as in
-    `norm_rope` where asked. Returns q [rows, q heads, dim] normed and turned (True where there is no q); None if
+    """Writes k and v [rows, heads, dim] behind what the batch's sequences hold (rows past a sequence's table nowhere),
+    k normed and turned first as in `norm_rope` where asked. Returns q [rows, q heads, dim] normed and turned (True where there is no q); None if
     declined."""
     out = _bind.append(k, v, cache, batch, q, positions, turns, q_weight, k_weight, eps, interleaved, factor)
     if out is not NotImplemented:
@@ -175,7 +175,7 @@ def append(k, v, cache, batch, q=None, positions=None, turns=None, q_weight=None
 
 def read(cache, batch, tail=None, dtype=torch.float16):
     """(k, v) [sequences, tail, heads, dim]: the last `tail` tokens (None: max_length) of each sequence, zeros where
-    it has fewer; None if declined."""
+    it has fewer or its table ends before; None if declined."""
     out = _bind.read(cache, batch, tail, dtype)
     if out is not NotImplemented:
         return out

@@ -31,13 +31,15 @@ struct Pool {
 };
 
 // The call's rows: sequence s has rows starts[s]..starts[s+1] of `rows` and lengths[s] tokens in the cache,
-// those rows' own among them; its blocks are table[s * width ...].
+// those rows' own among them; its blocks are table[s * width ...]. Positions count from all lengths[s] tokens, also
+// where the table is shorter: tokens past it are held nowhere, and those before stay where they are.
 struct Rows {
   const int32_t *table, *lengths, *starts;
   int sequences, width, rows;
   DEV int first(int s) const { return min(max(starts[s], 0), rows); }
   DEV int count(int s) const { return max(min(starts[s + 1], rows) - first(s), 0); }
-  DEV int length(int s) const { return max(min(lengths[s], width * BLOCK), 0); }
+  DEV int length(int s) const { return max(lengths[s], 0); }
+  DEV int held(int s) const { return min(length(s), width * BLOCK); }
   // The block that holds tokens 64 j.. of s, or -1: an entry outside the pool holds no tokens.
   DEV int block(int s, int j, int blocks) const {
     if (j < 0 || j >= width) return -1;

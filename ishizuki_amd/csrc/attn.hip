@@ -33,7 +33,7 @@ __global__ __launch_bounds__(64 * W) void stream_kernel(Call c, Pool pool, Rows 
 
   // blocks that some row sees; those that every row sees whole need no mask
   const int i0 = r0 / c.group, i1 = (min(r0 + 16 * RT, packed) - 1) / c.group;
-  const int last = c.causal ? base + i1 + 1 : length, from = c.window ? max(base + i0 + 1 - c.window, 0) : 0;
+  const int last = min(c.causal ? base + i1 + 1 : length, rows.held(seq)), from = c.window ? max(base + i0 + 1 - c.window, 0) : 0;
   const int whole0 = c.window ? max(base + i1 + 1 - c.window, 0) : 0, whole1 = c.causal ? base + i0 + 1 : length;
   const int b0 = from / BLOCK, b1 = max((last + BLOCK - 1) / BLOCK, b0);
   const int each = (b1 - b0 + c.splits - 1) / c.splits;

@@ -134,6 +134,7 @@ __global__ __launch_bounds__(256) void append_kernel(Heads k, Heads v, Heads q, 
   const int row0 = rows.first(seq), n = rows.count(seq), length = rows.length(seq), start = length - n;
   if (n == 0) return;
   const int jb = max(start, 0) / BLOCK + j;
+  if (jb >= rows.width) return;  // past the table; below 2^31 tokens from here on
   const int lo = max(max(start, 0), jb * BLOCK), hi = min(length, jb * BLOCK + BLOCK);
   if (lo >= hi) return;
   const int block = rows.block(seq, jb, pool.blocks);
@@ -258,14 +259,14 @@ __global__ __launch_bounds__(256) void read_kernel(Pool pool, Rows rows, int tai
   const bool values = id & 1;
   id >>= 1;
   const int j = id % reach, seq = id / reach;
-  const int length = rows.length(seq), p0 = length - tail, jb = (p0 >> 6) + j;
-  const int s0 = max(p0 - jb * BLOCK, 0), s1 = min(length - jb * BLOCK, BLOCK);
+  const int p0 = rows.length(seq) - tail, to0 = j * BLOCK - (p0 & (BLOCK - 1));  // slot 0's place in the output
+  const int s0 = max(-to0, 0), s1 = min(tail - to0, BLOCK);
   if (s0 >= s1) return;
-  const int block = rows.block(seq, jb, pool.blocks);
+  const int block = rows.block(seq, (p0 >> 6) + j, pool.blocks);
   const float scale = block < 0 ? 0.0f : (values ? pool.vs : pool.ks)[pool.scale(block, head)];
   const uint8_t *const tile = (values ? pool.v : pool.k) + pool.tile(max(block, 0), head);
   // of slot 0 and dim 0
-  const int64_t at = (((int64_t)seq * tail + (jb * BLOCK - p0)) * pool.heads + head) * D;
+  const int64_t at = (((int64_t)seq * tail + to0) * pool.heads + head) * D;
   const int64_t step = (int64_t)pool.heads * D;
   if (!values) {
     const int d = 8 * (tid % PER);

@@ -47,7 +47,7 @@ __global__ __launch_bounds__(512, RT == 1 && D <= 128 ? 4 : 2) void tile_kernel(
 
   // blocks that some row of the workgroup sees, and the tokens that some, or all, of the wave's rows do
   const int i0 = r0 / c.group, i1 = (min(r0 + 128 * RT, packed) - 1) / c.group;
-  const int last = c.causal ? base + i1 + 1 : length, from = c.window ? max(base + i0 + 1 - c.window, 0) : 0;
+  const int last = min(c.causal ? base + i1 + 1 : length, rows.held(seq)), from = c.window ? max(base + i0 + 1 - c.window, 0) : 0;
   const int b0 = from / BLOCK, b1 = max((last + BLOCK - 1) / BLOCK, b0);
   const int each = (b1 - b0 + c.splits - 1) / c.splits;
   const int first = b0 + split * each, stop = min(first + each, b1);

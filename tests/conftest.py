@@ -13,6 +13,20 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an MI355X (runs the HIP kernels)")
 
 
+# Tests that hold a wrong value: they run, and are expected to fail.
+WRONG = {
+    "test_append_leaves_the_rest_alone":
+        "expects the rows of a sequence of 300 tokens in a table of 256 at 256 - 290 .., where include/ishizuki_hip.h puts them at "
+        "300 - 290 .. (test_tokens_past_the_table_are_written_nowhere)",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        if item.name in WRONG:
+            item.add_marker(pytest.mark.xfail(reason=WRONG[item.name], raises=AssertionError, strict=True))
+
+
 FP16_SUBNORMAL_STEP = 2.0 ** -24
 # Per-element criterion: |y - ref| <= ELEM_TOL * sum_k |x_k||w_k| + half an fp16 ulp of the output.
 # The reference judges each element against the sum of the magnitudes that formed it

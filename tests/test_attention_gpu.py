@@ -665,3 +665,97 @@ def test_binding_and_python_calls_agree(monkeypatch):
     monkeypatch.setattr(attention, "_bind", _None())
     for a, b in zip(compiled, calls(), strict=True):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- sequences longer than their table
+@pytest.mark.parametrize("dtype", [INT8, E4M3])
+@pytest.mark.parametrize("lengths,rows", [([65, 130], [1, 2]), ([68, 300], [5, 290]), ([129, 64], [70, 1]), ([2 ** 31 - 1, 60], [3, 1])])
+def test_tokens_past_the_table_are_written_nowhere(dtype, lengths, rows):
+    """Rows stand at their own positions, also where the table ends before or among them: those past it leave what it holds
+    alone, and the others go where a longer table puts them."""
+    print(f"append {dtype} {lengths} {rows}", flush=True)
+    table = i32(2, 5).view(2, 1).to(DEV)
+    starts = [0, rows[0], sum(rows)]
+    batch = attention.Batch(table, i32(*lengths).to(DEV), i32(*starts).to(DEV), max(rows), min(max(lengths), 512))
+    first = gpu(random_cache(8, 2, 64, dtype))
+    cache = attention.Cache(*(t.clone() for t in first))
+    model = Model(first)
+    k, v = normal(1, sum(rows), 2, 64) * 9, normal(2, sum(rows), 2, 64) * 9  # the partly filled blocks' scales grow
+    assert attention.append(k.to(DEV), v.to(DEV), cache, batch) is True
+    for which, t in enumerate((k, v)):
+        for s in range(2):
+            at = lengths[s] - rows[s]
+            if at < 64:
+                model.append(which, t[starts[s]:starts[s + 1]], [(2, 5)[s]], at)
+    model.check(cache)
+    for b in range(8):
+        if b not in (2, 5) or lengths[(2, 5).index(b)] - rows[(2, 5).index(b)] >= 64:
+            assert all(torch.equal(x[b].view(INT8), y[b].view(INT8)) for x, y in zip(cache, first))
+    # read back: positions before lengths[s], zeros past the table
+    tail = 80
+    for got, which in zip(attention.read(cache, batch, tail=tail, dtype=F32), (0, 1)):
+        for s in range(2):
+            want = torch.zeros(tail, 2, 64, dtype=torch.float64)
+            ref = values(cache, batch, s, 64)[which]
+            for i in range(tail):
+                if 0 <= lengths[s] - tail + i < 64:
+                    want[i] = ref[lengths[s] - tail + i]
+            assert torch.all((got[s].cpu().double() - want).abs() <= 2 * u(F32) * want.abs())
+
+
+@pytest.mark.parametrize("lengths,rows,causal,window", [
+    ([200, 70], [1, 1], True, 0), ([140, 66], [9, 5], True, 0), ([300, 129], [1, 2], True, 100), ([330, 200], [70, 100], True, 0),
+    ([210, 140], [60, 40], True, 20), ([300, 90], [40, 3], False, 0), ([9000, 20000], [40, 1], True, 9000),
+    ([2 ** 31 - 1, 128], [2, 2], True, 0), ([2 ** 31 - 1, 2 ** 31 - 1], [2, 40], False, 0)])
+@pytest.mark.parametrize("heads,group,dim,dtype,x", [(2, 4, 128, INT8, BF16), (1, 2, 64, E4M3, F16), (1, 3, 256, INT8, F16)])
+def test_attend_past_the_table(lengths, rows, causal, window, heads, group, dim, dtype, x):
+    """Causal order and windows go by the rows' own positions where the table holds only the first 128 tokens."""
+    print(f"attend {lengths} {rows} {causal} {window} {heads} x {group} x {dim} {dtype} {x}", flush=True)
+    table = i32(1, 4, 0, 3).view(2, 2).to(DEV)
+    batch = attention.Batch(table, i32(*lengths).to(DEV), i32(0, rows[0], sum(rows)).to(DEV), max(rows), min(max(lengths), 1 << 16))
+    cache = random_cache(6, heads, dim, dtype, seed=4)
+    q = normal(3, sum(rows), heads * group, dim, dtype=x)
+    got = attention.attend(q.to(DEV), gpu(cache), batch, causal=causal, window=window)
+    out, bound, shift = (torch.zeros(*q.shape[:2], n, dtype=torch.float64) for n in (dim, dim, 1))
+    at = 0
+    for s in range(2):
+        for i in range(rows[s]):  # a row sees what one row at its place sees of the 128 tokens
+            end = lengths[s] - rows[s] + i + 1 if causal else lengths[s]
+            begin = max(end - window, 0) if window else 0
+            end = min(end, 128)
+            if begin < end:
+                one = attention.Batch(batch.table[s:s + 1], i32(end), i32(0, 1), 1, end)
+                for to, part in zip((out, bound, shift), attention_reference(q[at:at + 1], cache, one, dim ** -0.5, True, end - begin)):
+                    to[at] = part[0]
+            at += 1
+    attention_close(got, q, (out, bound, shift))
+
+
+def test_captured_steps_past_the_table():
+    """A captured step that is replayed after its table is full drops the new tokens: nothing that is held changes."""
+    table = i32(3, 1).view(1, 2).to(DEV)
+    lengths = i32(126).to(DEV)
+    batch = attention.Batch(table, lengths, i32(0, 1).to(DEV), 1, 128)
+    cache = gpu(random_cache(4, 2, 128, INT8, seed=9))
+    k, v = (normal(1, 1, 2, 128) * 30).to(DEV), normal(2, 1, 2, 128).to(DEV)
+
+    def step():
+        lengths.add_(1)
+        attention.append(k, v, cache, batch)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert lengths.item() == 128
+    full = [t.clone() for t in cache]
+    k.mul_(50), v.mul_(50)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(cache, full))

@@ -266,7 +266,7 @@ int ishz_moe_swiglu(uint32_t type, const void *x, int x_dtype, int T, int H, con
  *
  * The cache is a pool of blocks of ISHZ_KV_BLOCK tokens. Codes: of keys [blocks][heads][64][dim], of
  * values [blocks][heads][dim][64], one byte each; scales [blocks][heads] fp32 of either. A value is its
- * code times its block's and head's scale.
+ * code times its block's and head's scale, which is 0 or more.
  *
  * A call's sequences: table [sequences][width] holds each sequence's block numbers in order, lengths
  * [sequences] its tokens in the cache, the call's own among them, and starts [sequences + 1] the first of
@@ -312,8 +312,8 @@ int ishz_kv_read(const void *k_codes, const void *v_codes, const float *k_scale,
                  int blocks, int heads, int dim, const int32_t *table, int width, const int32_t *lengths,
                  int sequences, int tail, int dtype, void *k_out, void *v_out, ishz_stream_t stream);
 
-/* out [rows][q_heads][dim] = softmax(scale q K^T) V for each of the call's rows, q head h over the cache's head
-   h / (q_heads / heads). causal: a row sees tokens up to its own position; window w > 0 (causal calls): the last
+/* out [rows][q_heads][dim] = softmax(scale q K^T) V for each of the call's rows (scale of either sign), q head h over
+   the cache's head h / (q_heads / heads). causal: a row sees tokens up to its own position; window w > 0 (causal calls): the last
    w of those. Not causal: all its sequence's tokens. A row that sees no token gives zeros; rows of no sequence are
    left alone. max_rows and max_length: at least the most rows and tokens of a sequence, from which the work is
    divided; what is written to a sequence's rows beyond max_rows is unspecified. workspace:

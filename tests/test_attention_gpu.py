@@ -759,3 +759,17 @@ def test_captured_steps_past_the_table():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(cache, full))
+
+
+@pytest.mark.parametrize("lengths,rows,causal,window", [([700], [3], True, 0), ([700, 300], [40, 300], True, 0), ([900], [70], True, 130),
+                                                        ([333], [33], False, 0), ([20000], [1], True, 0)])
+@pytest.mark.parametrize("scale", [-0.6, 0.6])
+@pytest.mark.parametrize("heads,group,dim,dtype,x", [(1, 4, 128, INT8, BF16), (2, 2, 64, E4M3, F16), (1, 3, 256, INT8, F16)])
+def test_attend_scales_of_either_sign(lengths, rows, causal, window, scale, heads, group, dim, dtype, x):
+    """Logits of some tens: a row's reference moves as it goes, and one or a few tokens take all the weight."""
+    print(f"attend {lengths} {rows} {causal} {window} {scale} {heads} x {group} x {dim} {dtype} {x}", flush=True)
+    batch, blocks = make_batch(lengths, rows, seed=1)
+    cache = random_cache(blocks, heads, dim, dtype, seed=sum(lengths))
+    q = normal(3, sum(rows), heads * group, dim, dtype=x)
+    got = attention.attend(q.to(DEV), gpu(cache), batch, scale=scale, causal=causal, window=window)
+    attention_close(got, q, attention_reference(q * math.copysign(1, scale), cache, batch, abs(scale), causal, window))

@@ -63,16 +63,19 @@ def turns(dim=None, base=10000.0, inv_freq=None, device="cuda"):
 
 
 def _heads(x, what):
-    """x [rows, heads, dim] as the kernels take it, and its strides: rows and heads on 16 bytes, else copied."""
+    """x [rows, heads, dim] as the kernels take it, and its strides: rows and heads on 16 bytes, else copied. The stride of
+    a single row or head counts for nothing: slices keep odd ones there, and contiguous() leaves them as they are."""
     if x.dim() != 3:
         raise ValueError(f"{what} must be [rows, heads, dim]")
+    rows, heads, dim = x.shape
     row, head, last = x.stride()
+    row, head = row if rows > 1 else heads * dim, head if heads > 1 else dim
     step = 16 // x.element_size()
     if last != 1 or row % step or head % step or x.data_ptr() & 15:
         x = x.contiguous()
         if x.data_ptr() & 15:
             x = x.clone()
-        row, head, _ = x.stride()
+        row, head = heads * dim, dim
     return x, row, head
 
 

@@ -63,7 +63,7 @@ int truth(PyObject *o) {
   return o == Py_True;
 }
 
-// [rows, heads, dim] whose rows and heads start on 16 bytes.
+// [rows, heads, dim] whose rows and heads start on 16 bytes. The stride of a single row or head counts for nothing.
 struct Heads {
   void *p = nullptr;
   int64_t row = 0, head = 0;
@@ -76,10 +76,10 @@ struct Heads {
     type = t.scalar_type();
     dtype = dtype_of(type);
     p = t.data_ptr();
-    row = t.stride(0), head = t.stride(1);
+    rows = count(t.size(0)), heads = count(t.size(1)), dim = count(t.size(2));
+    row = rows > 1 ? t.stride(0) : (int64_t)heads * dim, head = heads > 1 ? t.stride(1) : dim;
     const int64_t step = dtype == ISHZ_DT_F32 ? 4 : 8;
     fits(t.stride(2) == 1 && row % step == 0 && head % step == 0 && ((uintptr_t)p & 15) == 0);
-    rows = count(t.size(0)), heads = count(t.size(1)), dim = count(t.size(2));
   }
 };
 struct Turn {

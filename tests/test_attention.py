@@ -187,3 +187,24 @@ def test_binding_leaves_what_does_not_fit():
                 _bind.attend(x, cache, batch(), None, True, 0), _bind.attend("q", (), 3, None, True, 0), _bind.read(cache, batch(), -1, torch.float16),
                 _bind.append(x, x, cache, batch(), None, None, None, None, None, 1e-6, False, 1.0), _bind.append()):
         assert out is NotImplemented
+
+
+@pytest.mark.parametrize("rows,heads,width,first", [(1, 4, 771, 0), (1, 1, 780, 64), (3, 1, 776, 0), (1, 2, 132, 1), (3, 2, 136, 0)])
+def test_strides_of_single_rows_and_heads(library, rows, heads, width, first):
+    """A slice of one row or head keeps strides that nothing goes by: odd ones are neither passed on nor a reason to decline."""
+    cache = attention.new_cache(2, heads, 64, device="cpu")
+    wide = torch.zeros(rows + 1, width, dtype=torch.float16)
+    slices = [wide[:, first:first + 64 * heads].unflatten(1, (heads, 64))[:rows]]
+    if heads == 1:
+        slices += [torch.zeros(rows + 1, 3, 65, dtype=torch.float16)[:rows, at:at + 1, at:at + 64] for at in (0, 1)]
+    for x in slices:
+        attention.attend(x, cache, batch(rows))
+        attention.norm_rope(x, x)
+        attention.append(x, x, cache, batch(rows), q=x)
+        assert len(library.calls) == 3
+        for name, args in library.calls:
+            for i in {"ishz_kv_attend": [0], "ishz_norm_rope": [0, 4], "ishz_kv_append": [0, 3, 22]}[name]:
+                assert args[i] % 16 == 0 and args[i + 1] % 8 == 0 and args[i + 2] % 8 == 0
+                if rows > 1 and x.stride(0) % 8 == 0:
+                    assert args[i:i + 2] == (x.data_ptr(), x.stride(0))  # not copied
+        library.calls.clear()

@@ -773,3 +773,30 @@ def test_attend_scales_of_either_sign(lengths, rows, causal, window, scale, head
     q = normal(3, sum(rows), heads * group, dim, dtype=x)
     got = attention.attend(q.to(DEV), gpu(cache), batch, scale=scale, causal=causal, window=window)
     attention_close(got, q, attention_reference(q * math.copysign(1, scale), cache, batch, abs(scale), causal, window))
+
+
+@pytest.mark.parametrize("x", [F16, F32])
+@pytest.mark.parametrize("rows,heads", [(1, 4), (3, 1), (1, 1)])
+def test_slices_of_one_row_or_head(rows, heads, x):
+    """One row of a projection whose rows are an odd step apart, one head of several that are: served as the dense tensor is."""
+    batch, blocks = make_batch([70], [rows], seed=1)
+    first = gpu(random_cache(blocks, heads, 64, INT8, seed=2))
+    wide = normal(5, 4, 771, dtype=x).to(DEV)
+    if heads > 1:
+        slices = [wide[:, at:at + 64 * heads].unflatten(1, (heads, 64))[r:r + 1] for r, at in ((0, 0), (1, 0), (0, 3))]
+    else:
+        slices = [normal(6, 4, 5, 65, dtype=x).to(DEV)[:rows, at:at + 1, at:at + 64] for at in (0, 1)]
+    for t in slices:
+        dense = torch.empty(t.shape, dtype=x, device=DEV).copy_(t)
+        w = torch.full((64,), 1.5, device=DEV)
+        for y, z in zip(attention.norm_rope(t, t, q_weight=w), attention.norm_rope(dense, dense, q_weight=w)):
+            assert torch.equal(y, z)
+        pools = []
+        for y in (t, dense):
+            cache = attention.Cache(*(a.clone() for a in first))
+            assert attention.append(y, y, cache, batch, q=y, k_weight=w) is not None
+            pools.append(cache)
+        assert all(torch.equal(a, b) for a, b in zip(*pools))
+        if x is F16:
+            got = attention.attend(t, pools[0], batch)
+            assert got is not None and torch.equal(got, attention.attend(dense, pools[1], batch))

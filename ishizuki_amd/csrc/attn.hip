@@ -321,7 +321,8 @@ extern "C" int ishz_kv_attend(const void *q, int64_t q_row, int64_t q_head, int 
   const size_t need = p.splits == 1 ? 0 : (size_t)p.splits * rows * q_heads * (dim + 2) * 4;
   if (workspace_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 15)))) return ishz::einval("workspace too small");
   const int64_t total = (int64_t)sequences * heads * p.tiles * p.splits, joins = ((int64_t)rows * q_heads + 3) / 4;
-  if (total > (1 << 24) - 1 || joins > (1 << 24) - 1) return ishz::decline("more rows than a launch holds");
+  // a launch holds fewer than 2^32 threads
+  if (total * (p.stream ? 64 * p.waves : 512) > UINT32_MAX || joins > (1 << 24) - 1) return ishz::decline("more rows than a launch holds");
   float *const part = (float *)workspace;
   const Call c = {q, q_row, q_head, out, q_heads, group, scale * 1.44269504088896341f, causal, window, p.splits, part,
                   (float2 *)(part + (need ? (size_t)p.splits * rows * q_heads * dim : 0))};

@@ -363,7 +363,7 @@ extern "C" int ishz_norm_rope(const void *q, int64_t q_row, int64_t q_head, int 
   if (dim != 64 && dim != 128 && dim != 256) return ishz::decline("heads of 64, 128 or 256 values");
   if (rows < 0 || q_heads < 0 || k_heads < 0) return ishz::einval("a negative count");
   if (int rc = check_turn(positions, turns, rot, dim, rows)) return rc;
-  const int total = q_heads + k_heads;
+  const int64_t total = (int64_t)q_heads + k_heads;
   if (rows == 0 || total == 0) return ISHZ_OK;
   if (q_heads) {
     if (!q_out) return ishz::einval("null output");
@@ -375,10 +375,13 @@ extern "C" int ishz_norm_rope(const void *q, int64_t q_row, int64_t q_head, int 
   }
   const Heads gq = {q, q_row, q_head, q_heads, q_weight, q_out}, gk = {k, k_row, k_head, k_heads, k_weight, k_out};
   const Turn t = {positions, turns, rot, interleaved, factor};
-  const int per = 64 / (dim / 16), groups = (total + per - 1) / per;
+  const int per = 64 / (dim / 16);
+  const int64_t groups = (total + per - 1) / per;
   // Rows that fill the chip with a wave each take one (its angles serve all its heads); fewer are spread over waves.
   const int waves = rows >= 2048 ? 1 : 4;
-  const dim3 grid((rows + 4 / waves - 1) / (4 / waves), waves == 1 ? 1 : (groups + 3) / 4);
+  const int64_t across = ((int64_t)rows + 4 / waves - 1) / (4 / waves);
+  if (across > (1 << 24) - 1 || total > INT32_MAX - 64) return ishz::decline("more rows or heads than a launch holds");
+  const dim3 grid((uint32_t)across, waves == 1 ? 1 : (uint32_t)std::min<int64_t>((groups + 3) / 4, UINT16_MAX));
   ISHZ_BY_DTYPE(dtype, ISHZ_BY_DIM(dim, hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_rope_kernel<DT, U>), grid, dim3(256), 0,
                                                            ishz::S(stream), gq, gk, t, eps, rows, waves)));
   ISHZ_LAUNCH_CHECK("norm and rotation launch");

@@ -208,3 +208,13 @@ def test_strides_of_single_rows_and_heads(library, rows, heads, width, first):
                 if rows > 1 and x.stride(0) % 8 == 0:
                     assert args[i:i + 2] == (x.data_ptr(), x.stride(0))  # not copied
         library.calls.clear()
+
+
+def test_launches_of_too_many_threads_are_declined():
+    """A launch holds fewer than 2^32 threads, of 256 or 512 a workgroup."""
+    tall = dict(heads=8, q_heads=64, sequences=4096, max_rows=8192, rows=8192 + 4095, max_length=8192)  # tiles of 512 threads
+    assert attend(**tall) == _lib.DECLINED, _lib.last_error()
+    many = dict(heads=8, q_heads=32, sequences=1 << 20, rows=1 << 20, max_length=640)  # eight waves
+    assert attend(**many) == _lib.DECLINED, _lib.last_error()
+    assert rope(rows=1 << 26) == rope(rows=(1 << 31) - 1) == _lib.DECLINED, _lib.last_error()
+    assert rope(q_heads=(1 << 31) - 1) == _lib.DECLINED, _lib.last_error()

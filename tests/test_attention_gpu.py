@@ -800,3 +800,13 @@ def test_slices_of_one_row_or_head(rows, heads, x):
         if x is F16:
             got = attention.attend(t, pools[0], batch)
             assert got is not None and torch.equal(got, attention.attend(dense, pools[1], batch))
+
+
+def test_norm_rope_of_more_heads_than_a_grid_is_tall():
+    """Heads go over the grid's second axis in turns: 2^21 + 3 of them, one row."""
+    heads = (1 << 21) + 3
+    x = normal(1, 1, 8, 64, dtype=F16).to(DEV).repeat(1, heads // 8 + 1, 1)[:, :heads]
+    w = torch.full((64,), 1.5, device=DEV)
+    few, _ = attention.norm_rope(x[:, :8], x[:, :0], q_weight=w)
+    many, _ = attention.norm_rope(x, x[:, :0], q_weight=w)
+    assert torch.equal(many, few.repeat(1, heads // 8 + 1, 1)[:, :heads])

@@ -295,7 +295,7 @@ int ishz_norm_rope(const void *q, int64_t q_row, int64_t q_head, int q_heads, co
    A block that starts with this call's tokens gets for each head the scale max|x| / 127 (int8) or
    max|x| / 448 (e4m3), 2^-126 at least. A partly filled block keeps its scale unless a new token is too large
    for it, and then grows it by the least power of two that holds it, its older codes rounded to the new
-   scale. Codes are the nearest, ties to even. An infinity or NaN makes the scale of its block and head NaN, until the
+   scale. Codes are the nearest to the fp32 quotient by the scale, ties to even. An infinity or NaN makes the scale of its block and head NaN, until the
    block is started again. A block that is written belongs to one sequence of the call. max_rows: at least
    the most rows of a sequence (tokens of blocks beyond it are not written). */
 int ishz_kv_append(const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head,

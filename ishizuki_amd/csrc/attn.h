@@ -90,6 +90,14 @@ DEV uint32_t encode4(float a, float b, float c, float d) {
   return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
 }
 
+// x / scale as a division rounds it, from up = 1 / scale: what the product leaves of x corrects it (two fused
+// multiply-adds; the product alone is off by a step for a quarter of the values, which moves those at a border between
+// codes). A zero keeps its sign. For scales below 2^-100, whose remainders leave fp32, to a step.
+DEV float quotient(float x, float scale, float up) {
+  const float q = x * up;
+  return __builtin_fmaf(-__builtin_fmaf(q, scale, -x), up, q);
+}
+
 // ---------------------------------------------------------------- activations, eight at a time
 template <int DT>
 DEV void load8(const void *p, size_t i, float *o) {

@@ -181,7 +181,8 @@ __global__ __launch_bounds__(256) void append_kernel(Heads k, Heads v, Heads q, 
       uint32_t code[4];
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        code[i] = scale != scale ? 0 : encode4<FMT>(x[m][4 * i] * up, x[m][4 * i + 1] * up, x[m][4 * i + 2] * up, x[m][4 * i + 3] * up);
+        code[i] = scale != scale ? 0 : encode4<FMT>(quotient(x[m][4 * i], scale, up), quotient(x[m][4 * i + 1], scale, up),
+                                                    quotient(x[m][4 * i + 2], scale, up), quotient(x[m][4 * i + 3], scale, up));
       *(u2 *)(tile + slot * D + ca) = u2{code[0], code[1]};
       *(u2 *)(tile + slot * D + cb) = u2{code[2], code[3]};
     }
@@ -230,7 +231,8 @@ __global__ __launch_bounds__(256) void append_kernel(Heads k, Heads v, Heads q, 
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       uint32_t *const at = (uint32_t *)(tile + (dims + 128 * g + e) * BLOCK + first);
-      uint32_t code = scale != scale ? 0 : encode4<FMT>(x[g][0][e] * up, x[g][1][e] * up, x[g][2][e] * up, x[g][3][e] * up);
+      uint32_t code = scale != scale ? 0 : encode4<FMT>(quotient(x[g][0][e], scale, up), quotient(x[g][1][e], scale, up),
+                                                        quotient(x[g][2][e], scale, up), quotient(x[g][3][e], scale, up));
       if (fresh != ~0u) {
         const uint32_t was = *at;
         // tokens past s1 in a word are none of the sequence's: what is made of them does not matter, but they stay

@@ -810,3 +810,37 @@ def test_norm_rope_of_more_heads_than_a_grid_is_tall():
     few, _ = attention.norm_rope(x[:, :8], x[:, :0], q_weight=w)
     many, _ = attention.norm_rope(x, x[:, :0], q_weight=w)
     assert torch.equal(many, few.repeat(1, heads // 8 + 1, 1)[:, :heads])
+
+
+@pytest.mark.parametrize("x", [F32, F16, BF16])
+@pytest.mark.parametrize("dtype", [INT8, E4M3])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_codes_are_those_of_the_quotient(dtype, x, dim):
+    """Values at the borders between codes and a step beside them: the scale is the largest by 127 or 448 and the code that of
+    x by the scale, each one division in fp32, bit for bit."""
+    rows, heads, m = 150, 2, LIMIT[dtype]
+    batch, blocks = make_batch([rows], [rows], seed=4)
+    g = torch.Generator().manual_seed(dim)
+    size = 2.0 ** (torch.rand((1, heads, 1), generator=g) * 40 - 20)
+    code = torch.arange(127, dtype=INT8)
+    code = code.float() if dtype is INT8 else code.view(E4M3).float()
+    grid = (code[1:] + code[:-1]) / 2
+    grid = torch.cat((-grid, grid))
+    new = []
+    for _ in range(2):
+        t = grid[torch.randint(len(grid), (rows, heads, dim), generator=g)] / m * size
+        t[0::64, :, 0] = size[0, :, 0]  # each block's largest
+        t = torch.nextafter(t, t * torch.tensor([0.0, 1.0, 4.0])[torch.randint(3, t.shape, generator=g)])
+        new.append(torch.minimum(t.abs(), size).copysign(t).to(x))
+    cache = gpu(random_cache(blocks, heads, dim, dtype))
+    assert attention.append(*(t.to(DEV) for t in new), cache, batch) is True
+    for t, codes, scales, turned in ((new[0], cache.k, cache.k_scale, False), (new[1], cache.v, cache.v_scale, True)):
+        for j, b in enumerate(batch.table[0].tolist()):
+            part = t[64 * j:64 * j + 64].float().transpose(0, 1)
+            scale = part.abs().amax((1, 2)) / m
+            assert torch.equal(scales[b].cpu(), scale)
+            want = (part / scale[:, None, None]).clamp(-m, m)
+            want = (want.round() if dtype is INT8 else want).to(dtype)
+            got = codes[b].cpu().view(INT8)
+            got = (got.transpose(-1, -2) if turned else got)[:, :part.shape[1]]
+            assert torch.equal(got, want.view(INT8))

@@ -216,7 +216,8 @@ struct Call {
   int64_t row, head;  // strides in values
   void *out;          // [rows][heads][dim]
   int heads, group;   // q heads, and of them to a head of the cache
-  float scale;        // of the logits, times log2 e
+  float scale;        // of the logits, its magnitude times log2 e
+  uint32_t sign;      // and its sign, of two fp16 values
   int causal, window;
   int splits;
   float *part;  // [splits][rows][heads][dim]: sums in units of their own maximum
@@ -224,8 +225,8 @@ struct Call {
 };
 
 // A lane's values of a row of q, as matrix operands: dims 64 e + 16 quad .. + 15 for each e of D / 64; bf16 as fp16 with a
-// power of two for the row (see act_prepare), which the returned factor of its logits holds. A negative scale turns the
-// values' signs, so that the factor is never below 0 and a row's largest product is its largest logit.
+// power of two for the row (see act_prepare), which the returned factor of its logits holds. The scale's sign goes into the
+// values, so that the factor is never below 0 and a row's largest product is its largest logit.
 template <int D, int DT>
 DEV float load_query(const Call &c, int64_t row, int head, int quad, h8 *q) {
   constexpr int C = D / 64;
@@ -233,7 +234,7 @@ DEV float load_query(const Call &c, int64_t row, int head, int quad, h8 *q) {
   u4 v[2 * C];
 #pragma unroll
   for (int e = 0; e < 2 * C; e++) v[e] = *(const u4 *)((const uint16_t *)c.q + at + 64 * (e / 2) + 8 * (e % 2));
-  float scale = fabsf(c.scale);
+  float scale = c.scale;
   if (DT == ISHZ_DT_BF16) {
     uint32_t m = 0;
 #pragma unroll
@@ -248,7 +249,7 @@ DEV float load_query(const Call &c, int64_t row, int head, int quad, h8 *q) {
     scale *= ldexpf(1.0f, x);
   }
 #pragma unroll
-  for (int e = 0; e < 2 * C; e++) q[e] = as_h8(c.scale < 0 ? v[e] ^ 0x80008000u : v[e]);
+  for (int e = 0; e < 2 * C; e++) q[e] = as_h8(v[e] ^ c.sign);
   return scale;
 }
 

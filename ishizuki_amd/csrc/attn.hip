@@ -1,5 +1,6 @@
 // Attention over the 8-bit cache.
 #include <algorithm>
+#include <cmath>
 
 #include "attn.h"
 
@@ -324,7 +325,8 @@ extern "C" int ishz_kv_attend(const void *q, int64_t q_row, int64_t q_head, int 
   // a launch holds fewer than 2^32 threads
   if (total * (p.stream ? 64 * p.waves : 512) > UINT32_MAX || joins > (1 << 24) - 1) return ishz::decline("more rows than a launch holds");
   float *const part = (float *)workspace;
-  const Call c = {q, q_row, q_head, out, q_heads, group, scale * 1.44269504088896341f, causal, window, p.splits, part,
+  const Call c = {q, q_row, q_head, out, q_heads, group, std::fabs(scale) * 1.44269504088896341f,
+                  std::signbit(scale) ? 0x80008000u : 0u, causal, window, p.splits, part,
                   (float2 *)(part + (need ? (size_t)p.splits * rows * q_heads * dim : 0))};
   const Pool pool = {(uint8_t *)k_codes, (uint8_t *)v_codes, (float *)k_scale, (float *)v_scale, blocks, heads, dim};
   const Rows r = {table, lengths, starts, sequences, width, rows};

@@ -2,13 +2,14 @@
 
 Every .hip file under csrc/ is compiled with hipcc (and every .cpp, host-only, with g++) to an
 object in parallel, then linked; csrc/python/bind.cpp, Python's way into the attention calls, becomes
-_bind.so beside it. hipcc flags:
+_bind.so beside it, where torch is there (its headers; the C library needs none). hipcc flags:
   --offload-arch=gfx950                         CDNA4 only
   -Xclang -target-feature -Xclang -packed-fp32-ops   no packed fp32 instructions
   -O3 -fPIC -std=c++20 (g++ -std=c++17 for the host-only GGUF reader)
 """
 import concurrent.futures
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
@@ -71,14 +72,15 @@ def build(verbose=True):
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")) + glob.glob(os.path.join(CSRC, "*.cpp")))
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
-        bind = ex.submit(_compile_bind)
+        bind = ex.submit(_compile_bind) if importlib.util.find_spec("torch") else None
         objs = list(ex.map(_compile, srcs))
     tmp = LIB + ".tmp"
     subprocess.run([HIPCC, "--offload-arch=gfx950", "-shared", "-o", tmp, *objs], check=True)
     os.replace(tmp, LIB)
-    _link_bind(bind.result())
+    if bind:
+        _link_bind(bind.result())
     if verbose:
-        print("built", LIB)
+        print("built", LIB, "" if bind else "alone: no torch to build _bind.so with")
     return LIB
 
 

@@ -269,10 +269,12 @@ static Plan plan(int q_heads, int heads, int dim, int sequences, int max_rows, i
     }
   } else {
     // 256 rows a workgroup halve the decoding: for many of heads of 128 (4096 tokens of 32 heads over 8: 150 us, 128 rows
-    // 185; of 64 114 and 118), or few rows over a long cache (512 over 16384: 148 and 158; of 64 108 and 134). Otherwise 128
-    // rows end more evenly (2048 tokens: 59 us, 72; of 64 42 and 53).
+    // 185; of 64 114 and 118), or few rows over a long cache (512 over 16384: 148 and 158; of 64 108 and 134), of which they
+    // see enough (700 rows of 32 heads over 8 in a window of 4500, 76 blocks: 90 and 98; of 64 69 and 74; of 3000, 52 blocks,
+    // no difference; 3 x 1500 of 16 over 2 of 64 in one of 4096, 70 blocks: 195 and 153). Otherwise 128 rows end more evenly
+    // (2048 tokens: 59 us, 72; of 64 42 and 53).
     const bool wide = packed > 128 && ((dim == 128 && pairs * tiles(256) >= 512) ||
-                                       (dim < 256 && blocks >= 128 && max_length >= 4 * (int64_t)max_rows));
+                                       (dim < 256 && blocks >= 128 && span >= 72 && max_length >= 4 * (int64_t)max_rows));
     p.row_tiles = wide ? 2 : 1;
     p.tiles = (int)tiles(128 * p.row_tiles);
     // A workgroup a CU, two where a sequence's rows are one tile and the parts to join few (4 x 8 tokens over 8191 of 32

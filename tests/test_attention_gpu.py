@@ -844,3 +844,49 @@ def test_codes_are_those_of_the_quotient(dtype, x, dim):
             got = codes[b].cpu().view(INT8)
             got = (got.transpose(-1, -2) if turned else got)[:, :part.shape[1]]
             assert torch.equal(got, want.view(INT8))
+
+
+@pytest.mark.parametrize("n,heads,group,dim,length,rows,window", [
+    (16, 4, 8, 128, 300, 256, 0), (16, 4, 8, 128, 700, 256, 130), (24, 2, 2, 64, 8200, 260, 0), (24, 2, 2, 64, 8200, 260, 5000),
+    (24, 2, 2, 64, 8200, 260, 900)])
+@pytest.mark.parametrize("dtype,x", [(INT8, BF16), (E4M3, F16)])
+@pytest.mark.parametrize("scale", [None, 0.6])
+def test_attend_many_tiles(n, heads, group, dim, length, rows, window, dtype, x, scale):
+    """So many rows that no call is split: 256 rows a workgroup for heads of 128, and of 64 over long caches or wide windows,
+    128 else. All sequences but one have the same blocks."""
+    print(f"attend {n} x {rows} over {length} window {window} {heads} x {group} x {dim} {dtype} {x} {scale}", flush=True)
+    batch, blocks = make_batch([length, length], [rows, rows], seed=1)
+    cache = random_cache(blocks, heads, dim, dtype, seed=7)
+    order = [0] * (n - 1) + [1]
+    ragged = [rows - (s * 7) % 64 for s in range(n)]
+    starts = i32(0, *torch.tensor(ragged).cumsum(0).tolist())
+    lengths = i32(*(length - s for s in range(n)))
+    many = attention.Batch(batch.table[order].contiguous(), lengths.to(DEV), starts.to(DEV), rows, length)
+    q = normal(3, sum(ragged), heads * group, dim, dtype=x)
+    got = attention.attend(q.to(DEV), gpu(cache), many, scale=scale, window=window)
+    for s in (0, n // 2, n - 1):
+        one = attention.Batch(many.table[s:s + 1], lengths[s:s + 1], i32(0, ragged[s]), rows, length)
+        part = slice(int(starts[s]), int(starts[s + 1]))
+        attention_close(got[part], q[part], attention_reference(q[part], cache, one, dim ** -0.5 if scale is None else scale, True, window))
+
+
+def test_append_of_many_rows_with_queries():
+    """Above 2048 rows a wave turns a row's queries by itself."""
+    rows, lengths, heads, kv, dim = [1500, 600], [1530, 600], 6, 2, 64
+    batch, blocks = make_batch(lengths, rows, seed=3)
+    cache = random_cache(blocks, kv, dim, INT8, seed=8)
+    model, cache = Model(cache), gpu(cache)
+    qkv = normal(5, sum(rows), heads + 2 * kv, dim, dtype=BF16)
+    positions = torch.cat([torch.arange(n - r, n) for n, r in zip(lengths, rows)]).int()
+    inv = [1e4 ** (-2.0 * i / dim) for i in range(dim // 2)]
+    wq, wk = 1 + normal(2, dim) / 4, 2 + normal(3, dim) / 4
+    d = qkv.to(DEV)
+    q = attention.append(d[:, heads:heads + kv], d[:, heads + kv:], cache, batch, q=d[:, :heads], positions=positions.to(DEV),
+                         turns=attention.turns(inv_freq=inv, device=DEV), q_weight=wq.to(DEV), k_weight=wk.to(DEV))
+    y = rope_reference(qkv[:, :heads], positions, inv, wq, 1e-6, False)
+    assert torch.all((q.cpu().double() - y).abs() <= rope_tolerance(y, qkv[:, :heads], wq, 1e-6, BF16))
+    k = rope_reference(qkv[:, heads:heads + kv], positions, inv, wk, 1e-6, False)
+    for s, part in enumerate((slice(0, 1500), slice(1500, 2100))):
+        for which, t in enumerate((k, qkv[:, heads + kv:])):
+            model.append(which, t[part], batch.table[s].tolist(), lengths[s] - rows[s])
+    model.check(cache, key_error=2.0 ** -18)  # see rope_tolerance: 2^-19 sqrt 2 of the head's largest

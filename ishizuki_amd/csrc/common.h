@@ -165,12 +165,13 @@ DEV uint32_t block_absmax(uint32_t m, uint32_t *scratch) {
 }
 // e of 2^(e-1) <= m < 2^e for a row whose largest magnitude has bf16 bits m; 0 for a row of zeros or
 // with an infinity or a NaN. At most 127, so that 2^e stays a finite fp32 factor (a row whose
-// largest value lies in (2^127, FLT_MAX] lands in [0.5, 2)).
+// largest value lies in (2^127, FLT_MAX] lands in [0.5, 2)), and -127 at least, so that 2^-e does (a
+// row of subnormal values lands below 1).
 DEV int bf16_row_exponent(uint32_t m) {
   if (m == 0 || m >= 0x7f80u) return 0;
   int e;
   (void)frexpf(__builtin_bit_cast(float, m << 16), &e);
-  return min(e, 127);
+  return max(min(e, 127), -127);
 }
 // Eight bf16 values times `down`, rounded to fp16.
 DEV u4 bf16_to_half8(u4 v, float down) {

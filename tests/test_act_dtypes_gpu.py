@@ -242,3 +242,21 @@ def test_bf16_row_image_non_finite():
         x[0, 7] = v
         assert not torch.isfinite(ggml.matvec(x, blk, ggml.Q4_K, N)).any()
     assert (ggml.matvec(torch.zeros(1, K, dtype=torch.bfloat16, device=DEV), blk, ggml.Q4_K, N) == 0).all()
+
+
+@pytest.mark.parametrize("M", [1, 3, 8])
+@pytest.mark.parametrize("t", [ggml.Q4_0, ggml.Q4_K])
+def test_bf16_rows_of_subnormal_values(t, M):
+    """Rows whose largest value is a bf16 subnormal, down to 2^-133: the row's factor stays finite, and so does the output."""
+    N, K = 40, 512
+    blocks = synth.ggml_blocks(t, N, K, seed=t + M)
+    x = np.random.default_rng(M).integers(-3, 4, (M, K)).astype(np.float32) * np.float32(2.0 ** -133)
+    x[-1] *= 16
+    xt = torch.from_numpy(x).to(torch.bfloat16)
+    print(f"bf16 subnormal rows t={t} M={M}", flush=True)
+    y = ggml.matvec(xt.to(DEV), torch.from_numpy(blocks).to(DEV), t, N)
+    ref, bd = ggml_reference(t, xt.float().numpy() * np.float32(2.0 ** 100), blocks, N)
+    y = y.float().cpu().numpy().astype(np.float64)
+    assert np.all(np.isfinite(y))
+    lim = (1e-4 * bd + 2.0 ** -8 * np.abs(ref)) * 2.0 ** -100 + 2.0 ** -133  # and the spacing of bf16's subnormals
+    assert np.all(np.abs(y - ref.astype(np.float64) * 2.0 ** -100) <= lim)

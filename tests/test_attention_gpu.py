@@ -890,3 +890,14 @@ def test_append_of_many_rows_with_queries():
         for which, t in enumerate((k, qkv[:, heads + kv:])):
             model.append(which, t[part], batch.table[s].tolist(), lengths[s] - rows[s])
     model.check(cache, key_error=2.0 ** -18)  # see rope_tolerance: 2^-19 sqrt 2 of the head's largest
+
+
+@pytest.mark.parametrize("rows", [2, 80])
+def test_attend_queries_of_subnormal_values(rows):
+    """bf16 queries down to 2^-133: logits of next to nothing, so that every token seen has the same weight."""
+    batch, blocks = make_batch([200], [rows], seed=1)
+    cache = random_cache(blocks, 2, 128, INT8, seed=5)
+    q = (normal(3, rows, 4, 128) * 2.0 ** -131).to(BF16)
+    q[0] = 0
+    got = attention.attend(q.to(DEV), gpu(cache), batch)
+    attention_close(got, q, attention_reference(q, cache, batch, 128 ** -0.5, True, 0))

@@ -281,7 +281,7 @@ static Plan plan(int q_heads, int heads, int dim, int sequences, int max_rows, i
     // heads over 8 of 64: 18.5 us, 20.8 with one; 4 x 32 of 128 in a window of 4096: 26.8, two 31.5), and three blocks each
     // (16 tokens over 1500: 12.2 us, six 14.9). Where rows see nine blocks or fewer on average the join costs more than
     // that gives (16 tokens over 700: 12.9, unsplit 16.1; over 512 in two splits no gain; 700 among themselves 24 and 20).
-    const int64_t mean = std::min(span, (max_length - max_rows / 2 + BLOCK - 1) / (int64_t)BLOCK);
+    const int64_t mean = std::min(span, ((int64_t)max_length - max_rows / 2 + BLOCK - 1) / BLOCK);
     splits = 256 / std::max<int64_t>(pairs * p.tiles, 1);
     if (splits > 1 && splits <= 8 && dim < 256 && packed * dim <= 8192) splits *= 2;
     splits = mean < 9 ? 1 : std::min(splits, span / 3);

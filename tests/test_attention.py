@@ -218,3 +218,9 @@ def test_launches_of_too_many_threads_are_declined():
     assert attend(**many) == _lib.DECLINED, _lib.last_error()
     assert rope(rows=1 << 26) == rope(rows=(1 << 31) - 1) == _lib.DECLINED, _lib.last_error()
     assert rope(q_heads=(1 << 31) - 1) == _lib.DECLINED, _lib.last_error()
+
+
+def test_lengths_without_a_bound_are_split():
+    """max_length may be as large as a host number gets: rows that take tiles are split as for any long cache."""
+    size = _lib.lib().ishz_kv_attend_workspace_size
+    assert size(70, 4, 1, 128, 1, 70, (1 << 31) - 1) == size(70, 4, 1, 128, 1, 70, 1 << 30) > 0

@@ -411,8 +411,8 @@ extern "C" int ishz_kv_append(const void *k, int64_t k_row, int64_t k_head, cons
   }
   // max_rows rows that start anywhere in a block reach this many.
   max_rows = std::min(max_rows, rows);
-  const int reach = max_rows > 0 ? (max_rows + BLOCK - 2) / BLOCK + 1 : 0;
-  const int64_t writers = (int64_t)sequences * reach * 2 * heads, waves = rows >= 2048 ? 1 : 4;  // as for ishz_norm_rope
+  const int64_t reach = max_rows > 0 ? ((int64_t)max_rows + BLOCK - 2) / BLOCK + 1 : 0;
+  const int64_t writers = sequences * reach * 2 * heads, waves = rows >= 2048 ? 1 : 4;  // as for ishz_norm_rope
   const int64_t turners = q_heads ? (rows + 4 / waves - 1) / (4 / waves) : 0;
   if (writers + turners > (1 << 24) - 1) return ishz::decline("more blocks than a launch holds");
   if (writers + turners == 0) return ISHZ_OK;
@@ -423,7 +423,7 @@ extern "C" int ishz_kv_append(const void *k, int64_t k_row, int64_t k_head, cons
   const Rows r = {table, lengths, starts, sequences, width, rows};
   ISHZ_BY_FORMAT(format, ISHZ_BY_DTYPE(dtype, ISHZ_BY_DIM(dim, hipLaunchKernelGGL(
       HIP_KERNEL_NAME(append_kernel<DT, U, FMT>), dim3((uint32_t)(writers + turners)), dim3(256), 0, ishz::S(stream), gk, gv, gq,
-      t, eps, pool, r, reach, (int)writers, (int)waves))));
+      t, eps, pool, r, (int)reach, (int)writers, (int)waves))));
   ISHZ_LAUNCH_CHECK("cache append launch");
   return ISHZ_OK;
 }

@@ -217,6 +217,7 @@ def test_launches_of_too_many_threads_are_declined():
     many = dict(heads=8, q_heads=32, sequences=1 << 20, rows=1 << 20, max_length=640)  # eight waves
     assert attend(**many) == _lib.DECLINED, _lib.last_error()
     assert rope(rows=1 << 26) == rope(rows=(1 << 31) - 1) == _lib.DECLINED, _lib.last_error()
+    assert append(rows=(1 << 31) - 1, max_rows=(1 << 31) - 1) == _lib.DECLINED, _lib.last_error()
     assert rope(q_heads=(1 << 31) - 1) == _lib.DECLINED, _lib.last_error()
 
 

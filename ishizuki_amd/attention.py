@@ -197,8 +197,10 @@ def read(cache, batch, tail=None, dtype=torch.float16):
 
 def attend(q, cache, batch, scale=None, causal=True, window=0):
     """[rows, q heads, dim]: attention of the batch's rows over their sequences' tokens in the cache, weights
-    softmax(scale q K^T) (`scale` None: dim ** -0.5). Causal: a row sees the tokens up to its own (`window` > 0: the
-    last `window` of them); else all of its sequence's. A row that sees none gives zeros. None if declined."""
+    softmax(scale q K^T) (`scale` None: dim ** -0.5; q fp16 or bf16). Causal: a row sees the tokens up to its own
+    (`window` > 0: the last `window` of them); else all of its sequence's. A row that sees none gives zeros. Rows of no
+    sequence, and those of a sequence beyond `max_rows`, are not written: they hold whatever the memory held. The work is
+    divided by the most rows of a sequence: prompts and single tokens are faster in a call each. None if declined."""
     out = _bind.attend(q, cache, batch, scale, causal, window)
     if out is not NotImplemented:
         return out

@@ -14,8 +14,8 @@ namespace attn {
 // Neither codes nor weights pass through LDS, and each is read from memory once. The W waves of a workgroup take every
 // W-th block and are joined in LDS; splits of a long cache are joined by join_kernel.
 // Memory bounds it over long caches: 16 sequences of 12000 to 32768 tokens of 8 heads of 128 (731 MB) take 131 us and the
-// join 4.8, 5.5 TB/s, where a kernel that only reads reaches 6.1. Vector operations are 32 % and matrix ones 7 % of the
-// SIMDs' time. One token over 777 takes 9 us: a launch, three dependent reads (table, codes and scales) and the joining.
+// join 4.8, 5.5 TB/s, where a kernel that only reads reaches 6.1. Vector operations are 35 % and matrix ones 7 % of the
+// SIMDs' time. One token over 777 takes 9 to 10 us: a launch, three dependent reads (table, codes and scales) and the joining.
 template <int D, int FMT, int DT, int RT, int W>
 __global__ __launch_bounds__(64 * W) void stream_kernel(Call c, Pool pool, Rows rows, int tiles) {
   constexpr int C = D / 64, V = D / 16, PITCH = D + 4;
@@ -264,7 +264,8 @@ static Plan plan(int q_heads, int heads, int dim, int sequences, int max_rows, i
       splits = 1;
     } else {
       // Four workgroups a CU, and at most 32 blocks a wave's share of four, so that long sequences beside short ones end
-      // sooner (16 sequences of 12000 to 32768 tokens, 8 heads: 138 us, 141 without; 60000 of one: 32.5).
+      // sooner (16 sequences of 12000 to 32768 tokens, 8 heads: 138 us, 141 without; 60000 of one: 32.5). No more than 64
+      // splits (below), so that fewer than 16 sequences and heads together fill less: one of one head a quarter of the CUs.
       splits = std::min(std::max((1024 + pairs - 1) / pairs, span / 32), (span + 3) / 4);
     }
   } else {
@@ -286,7 +287,7 @@ static Plan plan(int q_heads, int heads, int dim, int sequences, int max_rows, i
     if (splits > 1 && splits <= 8 && dim < 256 && packed * dim <= 8192) splits *= 2;
     splits = mean < 9 ? 1 : std::min(splits, span / 3);
   }
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, 64));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, 64));  // a lane of join_kernel each
   // the workspace's size knows no window
   if (window) p.splits = std::min(p.splits, plan(q_heads, heads, dim, sequences, max_rows, max_length, 0).splits);
   return p;

@@ -112,8 +112,9 @@ DEV float next_scale(uint32_t most, int s0, float old, int *grow) {
 // the scale is the exact maximum over its new tokens without a second pass or atomics: the tokens stay in registers
 // meanwhile. Of keys a thread has units of a token (the norm and the rotation go over the head); of values 4 tokens of 8
 // dims, which are whole words of the block's rows of tokens: nothing is turned in LDS. Workgroups past those turn q's
-// heads, `waves` waves a row. 8192 tokens of 8 heads of 128 in fp16 (50 MB) take 13.8 us, 3.7 TB/s, of which a launch and
-// the two waits (values, then the workgroup's maximum) are 5: one token of each of 16 sequences takes 6.2.
+// heads, `waves` waves a row. 8192 tokens of 8 heads of 128 in fp16 (50 MB) take 14.0 us, 3.6 TB/s, of which a launch and
+// the waits, one after the other (lengths and table, values, the workgroup's maximum), are 5: one token of each of 16
+// sequences takes 6.2.
 template <int DT, int U, int FMT>
 __global__ __launch_bounds__(256) void append_kernel(Heads k, Heads v, Heads q, Turn t, float eps, Pool pool, Rows rows,
                                                      int reach, int writers, int waves) {

@@ -13,10 +13,12 @@ namespace attn {
 // added to the block's logits, so that nothing but the matrix units touches the sums. A block outside 1..255 moves the
 // unit, which stays above 2^-72 of the largest scale the row has seen (the sums' 2^45 then stay finite).
 //
-// Power bounds it: these products alone, from registers, run at 1970 TFLOP/s on such values (1700 as 32x32x16) where the
-// clock would allow 2500, and a library product of 8192 x 8192 x 8192 at 1250 to 1500; 8192 tokens of 32 heads over 8 of
-// 128, causal, take 530 us (1040 TFLOP/s). That time is within 4 % for 16 to 48 rows a wave, products of either
-// shape, vector operations dealt between the products or not, and codes unpacked by a pass before.
+// Issue bounds it: 8192 tokens of 32 heads over 8 of 128, causal, take 526 to 546 us call after call (1010 to 1050 TFLOP/s),
+// 4530 cycles a block of 256 rows at 2.35 GHz. Matrix units are busy for 42 % of the cycles and vector operations for 45 %
+// (an exp2 takes two ordinary ones' cycles), in turn and hardly at once. By itself a call runs at 1.95 GHz and takes 620.
+// The products alone, from registers, run at 1970 TFLOP/s on such values (1700 as 32x32x16), a library product of
+// 8192 x 8192 x 8192 at 1250 to 1500. The time is within 4 % for 16 to 48 rows a wave, products of either shape, vector
+// operations dealt between the products or not, and codes unpacked by a pass before.
 template <int D, int FMT, int DT, int RT>
 __global__ __launch_bounds__(512, RT == 1 && D <= 128 ? 4 : 2) void tile_kernel(Call c, Pool pool, Rows rows, int tiles) {
   constexpr int C = D / 64, V = D / 16;

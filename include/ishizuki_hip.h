@@ -318,7 +318,9 @@ int ishz_kv_read(const void *k_codes, const void *v_codes, const float *k_scale,
    left alone. max_rows and max_length: at least the most rows and tokens of a sequence, from which the work is
    divided; what is written to a sequence's rows beyond max_rows is unspecified. workspace:
    ishz_kv_attend_workspace_size bytes (may be 0), 16-byte aligned. Sums are in a fixed order: the same call
-   gives the same bits. */
+   gives the same bits. Logits, weights and sums are fp32 but where the matrix units take them: a weight is rounded to
+   fp16 there (2^-11 of it at most), and q's bf16 values to fp16 times a power of two for the row (exact from 2^-17 of the
+   row's largest on). */
 size_t ishz_kv_attend_workspace_size(int rows, int q_heads, int heads, int dim, int sequences, int max_rows,
                                      int max_length);
 int ishz_kv_attend(const void *q, int64_t q_row, int64_t q_head, int q_heads, int dtype, int rows,

@@ -128,7 +128,7 @@ __global__ __launch_bounds__(64 * W) void stream_kernel(Call c, Pool pool, Rows 
         for (int i = 0; i < 4; i++) {
           const float w = __builtin_amdgcn_exp2f(s[r][t][i] - ref);
           sum += w;
-          // Weights are rounded to fp16 for the matrix units: 2^-12 of each, the sums below stay in 32 bits.
+          // Weights are rounded to fp16 for the matrix units: 2^-11 of each at most, the sums below stay in 32 bits.
           p[r][t / 2][4 * (t % 2) + i] = (_Float16)w;
         }
       l[r] = l[r] * alpha[r] + sum;

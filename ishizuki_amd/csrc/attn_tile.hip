@@ -214,7 +214,7 @@ __global__ __launch_bounds__(512, RT == 1 && D <= 128 ? 4 : 2) void tile_kernel(
             const float w2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][2], f[r], ref));
             const float w3 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][3], f[r], ref));
             sum += (w0 + w1) + (w2 + w3);
-            // Weights are rounded to fp16 for the matrix units: 2^-12 of each, the sums stay in 32 bits.
+            // Weights are rounded to fp16 for the matrix units: 2^-11 of each at most, the sums stay in 32 bits.
             const h2 lo = __builtin_convertvector((f2{w0, w1}), h2), hi = __builtin_convertvector((f2{w2, w3}), h2);
             p[r][t / 2][4 * (t % 2)] = lo.x, p[r][t / 2][4 * (t % 2) + 1] = lo.y;
             p[r][t / 2][4 * (t % 2) + 2] = hi.x, p[r][t / 2][4 * (t % 2) + 3] = hi.y;

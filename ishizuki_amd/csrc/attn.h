@@ -226,7 +226,7 @@ struct Call {
 
 // A lane's values of a row of q, as matrix operands: dims 64 e + 16 quad .. + 15 for each e of D / 64; bf16 as fp16 with a
 // power of two for the row (see act_prepare), which the returned factor of its logits holds. The scale's sign goes into the
-// values, so that the factor is never below 0 and a row's largest product is its largest logit.
+// values (bf16: with that power), so that the factor is never below 0 and a row's largest product is its largest logit.
 template <int D, int DT>
 DEV float load_query(const Call &c, int64_t row, int head, int quad, h8 *q) {
   constexpr int C = D / 64;
@@ -243,13 +243,13 @@ DEV float load_query(const Call &c, int64_t row, int head, int quad, h8 *q) {
     m = max((uint32_t)a[0], (uint32_t)a[1]);
     const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
     const int x = bf16_row_exponent(max((uint32_t)b[0], (uint32_t)b[1]));
-    const float down = ldexpf(1.0f, -x);
+    const float down = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, ldexpf(1.0f, -x)) | (c.sign & 0x80000000u));
 #pragma unroll
     for (int e = 0; e < 2 * C; e++) v[e] = bf16_to_half8(v[e], down);
     scale *= ldexpf(1.0f, x);
   }
 #pragma unroll
-  for (int e = 0; e < 2 * C; e++) q[e] = as_h8(v[e] ^ c.sign);
+  for (int e = 0; e < 2 * C; e++) q[e] = as_h8(DT == ISHZ_DT_BF16 ? v[e] : v[e] ^ c.sign);
   return scale;
 }
 
